@@ -34,6 +34,12 @@ class PeerOut(C.Structure):
                 ("seq", _I)]
 
 
+class Ffn(C.Structure):
+    """glmx_ffn of include/glmx.h"""
+    _fields_ = [("hidden", _I), ("intermediate", _I), ("dtype", _I), ("w_gate", _P), ("w_up", _P), ("w_down", _P),
+                ("act_limit", C.c_float)]
+
+
 class GlmxError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"glmx error {code}: {msg}")
@@ -47,10 +53,13 @@ EXPORTS = ("glmx_version", "glmx_last_error", "glmx_layer_create", "glmx_layer_d
            "glmx_moe_forward_hc_mix", "glmx_hc_apply_partials", "glmx_hc_finalize_norm",
            "glmx_selftest_bounded_wait", "glmx_router", "glmx_moe_forward_peer", "glmx_peer_reduce", "glmx_ep_split", "glmx_ipc_alloc",
            "glmx_ipc_free", "glmx_ipc_handle", "glmx_ipc_open", "glmx_ipc_close", "glmx_layer_device", "glmx_check_noalloc",
-           "glmx_ep_pack", "glmx_ep_unpack_add")
+           "glmx_ep_pack", "glmx_ep_unpack_add", "glmx_ffn_forward", "glmx_ffn_backward", "glmx_quantize_rows",
+           "glmx_linear_i8", "glmx_sample", "glmx_dense_check")
 IPC_HANDLE_BYTES = 64
 NOALLOC_SCRATCH_BYTES = 48 << 20
 ROUTER_MAX_EXPERTS = 512
+I8_MAX_K = 131056
+SAMPLE_MAX_VOCAB = 393216
 
 _lib = None
 
@@ -125,6 +134,19 @@ def load(path: str = LIB_PATH):
     L.glmx_ipc_open.restype = _I
     L.glmx_ipc_close.argtypes = [_P]
     L.glmx_ipc_close.restype = _I
+    _LL, _F = C.c_longlong, C.c_float
+    L.glmx_ffn_forward.argtypes = [C.POINTER(Ffn), _P, _LL, _I, _P, _LL, _I, _I, _P, _P, _P, _P]
+    L.glmx_ffn_forward.restype = _I
+    L.glmx_ffn_backward.argtypes = [C.POINTER(Ffn), _P, _LL, _P, _LL, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+    L.glmx_ffn_backward.restype = _I
+    L.glmx_quantize_rows.argtypes = [_P, _I, _LL, _I, _I, _P, _LL, _P, _P]
+    L.glmx_quantize_rows.restype = _I
+    L.glmx_linear_i8.argtypes = [_P, _LL, _P, _I, _I, _I, _P, _LL, _P, _P, _P, _LL, _I, _P]
+    L.glmx_linear_i8.restype = _I
+    L.glmx_sample.argtypes = [_P, _I, _LL, _I, _I, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _I, _P]
+    L.glmx_sample.restype = _I
+    L.glmx_dense_check.argtypes = [_P, C.POINTER(_I)]
+    L.glmx_dense_check.restype = _I
     if L.glmx_version() != ABI_VERSION:
         raise RuntimeError(f"libglmx ABI {L.glmx_version()} != {ABI_VERSION}")
     _lib = L

@@ -1,0 +1,178 @@
+"""Gated feed-forward block over dense 16-bit weights (glmx_ffn_forward / glmx_ffn_backward): an unquantised shared expert
+beside MoELayer's trellis experts, or one of the model's dense layers.
+
+    g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L), y = h Wd^T        (L = act_limit; 0: no clamp)
+
+`GatedFFN` is the block at inference, and its forward_train / backward pair the explicit form of a training step (the one
+to capture into a graph); `gated_ffn` is the same as a differentiable function.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .layer import _dt, _stream_ptr
+
+
+def _on(device: torch.device, stream):
+    """The context in which a call allocates and launches: tensors' device current, and `stream` (if given) current too,
+    so that its temporaries belong to the stream that uses them."""
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"stream on {stream.device}, tensors on {device}")
+        return torch.cuda.stream(stream)
+    if device.index != torch.cuda.current_device():
+        return torch.cuda.device(device)
+    return contextlib.nullcontext()
+
+
+def _rows(t: torch.Tensor, align: int) -> torch.Tensor:
+    """t [R, n] as rows of packed elements whose distance is a multiple of `align` elements and whose start is 16-byte
+    aligned; copied where it is not."""
+    if t.stride(1) != 1 or t.stride(0) % align or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
+        if t.shape[0] == 1 and t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.shape[1] % align == 0:
+            return t.as_strided(t.shape, (t.shape[1], 1))
+        n = t.shape[1]
+        pitch = (n + align - 1) // align * align
+        c = torch.empty((t.shape[0], pitch), dtype=t.dtype, device=t.device)[:, :n]
+        c.copy_(t)
+        return c
+    return t
+
+
+class GatedFFN:
+    """w_gate, w_up [I, H], w_down [H, I]: bf16 or fp16 CUDA tensors of one dtype, H and I multiples of 8; act_limit as
+    MoELayer's. The weights are used in place (copied once where not contiguous)."""
+
+    def __init__(self, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, act_limit: float = 0.0):
+        self.lib = _lib.load()
+        if w_gate.dim() != 2 or w_up.shape != w_gate.shape or tuple(w_down.shape) != tuple(w_gate.shape[::-1]):
+            raise ValueError("weights must be w_gate [I, H], w_up [I, H], w_down [H, I]")
+        self.I, self.H = int(w_gate.shape[0]), int(w_gate.shape[1])
+        if self.H < 8 or self.I < 8 or self.H % 8 or self.I % 8:
+            raise ValueError("H and I must be positive multiples of 8")
+        self.dtype, self.device = w_gate.dtype, w_gate.device
+        if self.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"weights must be bf16 or fp16, not {self.dtype}")
+        for w in (w_gate, w_up, w_down):
+            if w.dtype != self.dtype or w.device != self.device:
+                raise ValueError("weights must share one dtype and device")
+        if self.device.type != "cuda":
+            raise ValueError("weights must be on a CUDA device (there is no CPU path)")
+        if not act_limit >= 0.0:
+            raise ValueError("act_limit must be 0 (none) or positive")
+        with _on(self.device, None):
+            pack = lambda w: w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+            self.w_gate, self.w_up, self.w_down = (pack(w.detach()) for w in (w_gate, w_up, w_down))
+        self.act_limit = float(act_limit)
+        self._desc = _lib.Ffn(self.H, self.I, _dt(w_gate), self.w_gate.data_ptr(), self.w_up.data_ptr(),
+                              self.w_down.data_ptr(), self.act_limit)
+        self._ref = C.byref(self._desc)
+
+    def _in(self, x: torch.Tensor, what: str) -> torch.Tensor:
+        if x.dim() < 1 or x.shape[-1] != self.H:
+            raise ValueError(f"{what} must be [..., {self.H}]")
+        if x.dtype != self.dtype:
+            raise TypeError(f"{what} must be {self.dtype}, not {x.dtype}")
+        if x.device != self.device:
+            raise ValueError(f"{what} on {x.device}, weights on {self.device}")
+        return x if x.dim() == 2 else x.reshape(-1, self.H)
+
+    def _forward(self, x, y, accumulate, h, p, q):
+        x = _rows(x, 8)
+        check(self.lib.glmx_ffn_forward(self._ref, x.data_ptr(), x.stride(0), x.shape[0], y.data_ptr(), y.stride(0), _dt(y),
+                                        int(accumulate), h.data_ptr(), p, q, _stream_ptr(None)))
+
+    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False,
+                stream=None) -> torch.Tensor:
+        """y [..., H] for x [..., H] of the block's dtype. out_dtype: the block's dtype (default) or fp32; out: a
+        contiguous tensor of x's shape to write instead, accumulate=True to add to it (a shared expert's output onto
+        MoELayer.forward's)."""
+        with _on(self.device, stream):
+            x2 = self._in(x, "x")
+            if out is None:
+                if accumulate:
+                    raise ValueError("accumulate needs out")
+                dt = self.dtype if out_dtype is None else out_dtype
+                if dt not in (self.dtype, torch.float32):
+                    raise TypeError(f"out_dtype must be {self.dtype} or fp32")
+                out = torch.empty(x.shape, dtype=dt, device=self.device)
+            else:
+                if out.shape != x.shape or not out.is_contiguous() or out.device != self.device or out.data_ptr() % 16:
+                    raise ValueError("out must be contiguous, 16-byte aligned, of x's shape and device")
+                if out.dtype not in (self.dtype, torch.float32) or (out_dtype is not None and out_dtype != out.dtype):
+                    raise TypeError(f"out must be {self.dtype} or fp32")
+            if x2.shape[0]:
+                h = torch.empty((x2.shape[0], self.I), dtype=self.dtype, device=self.device)
+                self._forward(x2, out.view(-1, self.H), accumulate, h, None, None)
+            return out
+
+    __call__ = forward
+
+    # ---- training -----------------------------------------------------------------------------------------------
+    def forward_train(self, x: torch.Tensor, stream=None):
+        """(y, saved): y as forward's, and what backward needs: the packed input rows, the hidden rows and two fp32 factors per hidden
+        value (10 bytes for each, beside x)."""
+        with _on(self.device, stream):
+            x2 = _rows(self._in(x, "x"), 8)
+            n = x2.shape[0]
+            y = torch.empty(x.shape, dtype=self.dtype, device=self.device)
+            h = torch.empty((n, self.I), dtype=self.dtype, device=self.device)
+            pq = torch.empty((2, n, self.I), dtype=torch.float32, device=self.device)
+            if n:
+                self._forward(x2, y.view(-1, self.H), False, h, pq[0].data_ptr(), pq[1].data_ptr())
+            return y, (x2, h, pq)
+
+    def backward(self, dy: torch.Tensor, saved, need=(True, True, True, True), stream=None):
+        """(dx, dw_gate, dw_up, dw_down) for dy [..., H] from forward_train's saved; None where need says so."""
+        with _on(self.device, stream):
+            dy2 = _rows(self._in(dy, "dy"), 8)
+            x, h, pq = saved
+            n = x.shape[0]
+            if dy2.shape[0] != n:
+                raise ValueError("dy must have the forward call's rows")
+            empty = lambda shape, want: torch.empty(shape, dtype=self.dtype, device=self.device) if want else None
+            dx = empty(dy.shape, need[0])
+            dwg, dwu, dwd = empty((self.I, self.H), need[1]), empty((self.I, self.H), need[2]), empty((self.H, self.I), need[3])
+            inner = any(need[:3]) and n
+            dgu = empty((2, n, self.I), inner)
+            ptr = lambda t: 0 if t is None else t.data_ptr()
+            check(self.lib.glmx_ffn_backward(self._ref, dy2.data_ptr(), dy2.stride(0) if n else self.H, x.data_ptr(),
+                                             x.stride(0) if n else self.H, n, h.data_ptr(), pq[0].data_ptr(), pq[1].data_ptr(),
+                                             dgu[0].data_ptr() if inner else 0, dgu[1].data_ptr() if inner else 0, ptr(dx),
+                                             ptr(dwg), ptr(dwu), ptr(dwd), _stream_ptr(None)))
+            return dx, dwg, dwu, dwd
+
+
+class _GatedFFNFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, act_limit):
+        ffn = GatedFFN(w_gate, w_up, w_down, act_limit)
+        if not any(ctx.needs_input_grad[:4]):
+            return ffn.forward(x)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gated_ffn: a differentiated call cannot be captured into a graph (an eager graph of the "
+                               "same leaves would tie the capture to another stream); capture GatedFFN.forward_train and "
+                               "GatedFFN.backward")
+        y, (x2, h, pq) = ffn.forward_train(x)
+        ctx.save_for_backward(x2, h, pq, w_gate, w_up, w_down)
+        ctx.act_limit = act_limit
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, h, pq, w_gate, w_up, w_down = ctx.saved_tensors
+        ffn = GatedFFN(w_gate, w_up, w_down, ctx.act_limit)
+        return (*ffn.backward(dy, (x2, h, pq), ctx.needs_input_grad[:4]), None)
+
+
+def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              act_limit: float = 0.0) -> torch.Tensor:
+    """The block as a differentiable function of x and its weights (once differentiable; not in a graph capture: see
+    GatedFFN.forward_train)."""
+    return _GatedFFNFunction.apply(x, w_gate, w_up, w_down, float(act_limit))

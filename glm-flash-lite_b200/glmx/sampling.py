@@ -1,0 +1,62 @@
+"""Sampling from the head's logits with given random numbers (glmx_sample): temperature, top-k, top-p and min-p per row.
+The counterpart of Router for the vocabulary: a selection over one row per token, all on the device."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .ffn import _on
+from .layer import _dt, _stream_ptr
+
+
+def _param(v, default, dtype, B: int, device, what: str):
+    """(tensor or None, its device address, the value for all rows)"""
+    if not isinstance(v, torch.Tensor):
+        return None, 0, default if v is None else v
+    if v.dim() == 0:
+        v = v.expand(B)
+    if tuple(v.shape) != (B,) or v.device != device:
+        raise ValueError(f"{what} must be a number or a tensor [{B}] on {device}")
+    if v.dtype != dtype or not v.is_contiguous():
+        v = v.to(dtype).contiguous()
+    return v, v.data_ptr(), default
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out_dtype=torch.int64,
+           stream=None) -> torch.Tensor:
+    """ids [B] (int64 or int32) for logits [B, V] (fp16, bf16 or fp32; any row distance) and u fp32 [B] in [0, 1).
+
+    Weights are exp((l - max) / temperature). The top_k largest logits stay (0: all; ties to the lower id); of those, in
+    descending order, each whose predecessors hold less than top_p of the weight left (1: all); of those, each with at
+    least min_p times the largest weight; the largest always. The pick is the lowest id at which the running sum of the
+    kept weights, in id order, exceeds u times their sum. temperature 0 picks the largest logit (the lowest id of equal
+    ones). -inf and NaN logits are never picked; a row without any other gives -1.
+
+    temperature, top_k, top_p and min_p: one number for all rows, or a tensor [B]."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [B, V] with V >= 1")
+    B, V = logits.shape
+    if V > _lib.SAMPLE_MAX_VOCAB:
+        raise ValueError(f"at most {_lib.SAMPLE_MAX_VOCAB} logits a row")
+    if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"logits must be fp16, bf16 or fp32, not {logits.dtype}")
+    dev = logits.device
+    if dev.type != "cuda":
+        raise ValueError("logits must be on a CUDA device (there is no CPU path)")
+    if out_dtype not in (torch.int64, torch.int32):
+        raise TypeError("out_dtype must be int64 or int32")
+    if u.dtype != torch.float32 or tuple(u.shape) != (B,) or u.device != dev:
+        raise ValueError(f"u must be fp32 [{B}] on {dev}")
+    with _on(dev, stream):
+        if logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
+            logits = logits.contiguous()
+        u = u if u.is_contiguous() else u.contiguous()
+        t, tp, t0 = _param(temperature, 1.0, torch.float32, B, dev, "temperature")
+        k, kp, k0 = _param(top_k, 0, torch.int32, B, dev, "top_k")
+        p, pp, p0 = _param(top_p, 1.0, torch.float32, B, dev, "top_p")
+        m, mp, m0 = _param(min_p, 0.0, torch.float32, B, dev, "min_p")
+        ids = torch.empty(B, dtype=out_dtype, device=dev)
+        check(_lib.load().glmx_sample(logits.data_ptr(), _dt(logits), max(logits.stride(0), V), B, V, u.data_ptr(), tp, t0, kp,
+                                      k0, pp, p0, mp, m0, ids.data_ptr(), _dt(ids), _stream_ptr(None)))
+        return ids

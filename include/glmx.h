@@ -280,6 +280,74 @@ GLMX_API int glmx_moe_forward_noalloc(const glmx_layer* layer, const void* x, in
  * reference. The layer's device must be current. */
 GLMX_API int glmx_check_noalloc(const glmx_layer* layer, int ntok, int topk, void* stream, int* flags);
 
+/* ---- the dense operators beside the routed experts ------------------------------------------------------------------
+ * No counterpart in the reference (its dense layers, its head and its sampler are exllamav3's). All of them take plain
+ * device pointers on the current device, allocate nothing and may be captured into a graph. Device-side waits are
+ * bounded; glmx_dense_check reads their error word. */
+
+/* A gated feed-forward block over dense 16-bit weights: an unquantised shared expert, or a dense layer.
+ *   g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L), y = h Wd^T      (L = act_limit; 0: no clamp)
+ * with the layer's clamp (glmx_layer_desc.act_limit). Products are summed in fp32; h is rounded to the block's dtype. */
+typedef struct
+{
+    int hidden, intermediate; /* H, I: positive multiples of 8 */
+    int dtype;                /* GLMX_BF16 or GLMX_F16: weights, x, h, y (unless y_dtype says fp32) and all gradients */
+    const void* w_gate;       /* device [I][H], 16-byte aligned, as are the others */
+    const void* w_up;         /* device [I][H] */
+    const void* w_down;       /* device [H][I] */
+    float act_limit;
+} glmx_ffn;
+
+/* y [ntok][H] (y_dtype: the block's dtype or GLMX_F32; accumulate = 1 adds to what y holds) from x [ntok] rows of H, ldx
+ * elements apart (a multiple of 8, at least H), y rows ldy apart (at least H). h: caller's scratch [ntok][I], 16-byte aligned; it holds the hidden
+ * rows afterwards. p, q: fp32 [ntok][I] or both NULL; with them the two factors of the backward pass are kept,
+ *   p = min(silu(g), L) * [|u| <= L],  q = clamp(u, -L, L) * silu'(g) * [silu(g) <= L]
+ * so that du = dh * p and dg = dh * q. */
+GLMX_API int glmx_ffn_forward(const glmx_ffn* ffn, const void* x, long long ldx, int ntok, void* y, long long ldy,
+                              int y_dtype, int accumulate, void* h, float* p, float* q, void* stream);
+
+/* Gradients of glmx_ffn_forward (accumulate = 0) for dy [ntok][H] (rows lddy apart), from the x, h, p and q of the forward call: dx
+ * [ntok][H], dw_gate / dw_up [I][H], dw_down [H][I], all in the block's dtype, rows packed; a NULL one is not computed.
+ * dg, du: caller's scratch [ntok][I] each in the block's dtype (the gradients of g and u afterwards), 16-byte aligned; not needed (NULL) where only
+ * dw_down is asked for. */
+GLMX_API int glmx_ffn_backward(const glmx_ffn* ffn, const void* dy, long long lddy, const void* x, long long ldx, int ntok,
+                               const void* h, const float* p, const float* q, void* dg, void* du, void* dx, void* dw_gate,
+                               void* dw_up, void* dw_down, void* stream);
+
+/* Rows to 8 bits: scale[t] = max |x[t]| / 127 (an fp32 quotient), q[t][k] = x[t][k] / scale[t] (an fp32 quotient) rounded
+ * to the nearest integer, ties to even; a row of zeros gets scale 0 and zeros. x: [rows] rows of K, ldx elements apart,
+ * fp16, bf16 or fp32, finite. q: int8, rows ldq bytes apart (ldq >= K; bytes K .. ldq - 1 of a row are left as they were). */
+GLMX_API int glmx_quantize_rows(const void* x, int x_dtype, long long ldx, int rows, int K, signed char* q, long long ldq,
+                                float* scale, void* stream);
+
+/* 8-bit matrix product: y[t][n] = (sum_k xq[t][k] * wq[n][k]) * (x_scale[t] * w_scale[n]) + bias[n], the sum in exact
+ * 32-bit integers. xq [ntok] rows and wq [N] rows of K int8, ldxq / ldwq bytes apart (multiples of 16, pointers
+ * 16-byte aligned; what lies behind K in a row is not read), bias fp32 [N] or NULL, y [ntok] rows of N, ldy elements apart, fp16, bf16 or
+ * fp32. 1 <= K <= GLMX_I8_MAX_K (a longer sum could pass 31 bits). */
+#define GLMX_I8_MAX_K 131056
+GLMX_API int glmx_linear_i8(const signed char* xq, long long ldxq, const float* x_scale, int ntok, int K, int N,
+                            const signed char* wq, long long ldwq, const float* w_scale, const float* bias, void* y,
+                            long long ldy, int y_dtype, void* stream);
+
+/* Picks a token for each row of logits [B] x V (rows ld elements apart; fp16, bf16 or fp32) from a given uniform number
+ * u[b] in [0, 1): with m the row's largest logit,
+ *   w_i = exp((l_i - m) / temperature); the top_k largest logits are kept (0 or less: all), ties to the lower id; of
+ *   those, in descending order, each whose predecessors hold less than top_p of the weight left (top_p >= 1: all); of
+ *   those, each with w_i >= min_p; the largest always. The pick is the lowest id at which the running sum of
+ *   the kept weights, in id order, exceeds u * their sum.
+ * temperature <= 0 picks the largest logit (ties to the lower id). A logit of -inf or NaN is never picked; a row that has no other gives -1.
+ * Equal +inf logits share the weight. temperature, top_k, top_p, min_p: device arrays [B], or NULL for the value behind
+ * (one for all rows). ids: [B] GLMX_I32 or GLMX_I64. Weights are exponentials in fp32 (a few ulp) rounded to multiples of
+ * 2^-44 and summed as 64-bit integers, so a call's result does not depend on the order of summation. */
+#define GLMX_SAMPLE_MAX_VOCAB 393216
+GLMX_API int glmx_sample(const void* logits, int dtype, long long ld, int B, int V, const float* u, const float* temperature,
+                         float temperature0, const int* top_k, int top_k0, const float* top_p, float top_p0,
+                         const float* min_p, float min_p0, void* ids, int ids_dtype, void* stream);
+
+/* Synchronises `stream` and reads the dense operators' device error word on the current device (a bounded wait that expired):
+ * GLMX_OK or GLMX_E_DEVICE; *flags receives the bits. The word is sticky; the call clears it. */
+GLMX_API int glmx_dense_check(void* stream, int* flags);
+
 #ifdef __cplusplus
 }
 #endif
