@@ -1,11 +1,71 @@
-// Error word of the dense operators (glmx_dense_check): one per device, sticky, set by a kernel whose bounded wait expired.
-#include "dense.h"
+// What the dense operators' launches share: tensor maps, device facts, and the error word (glmx_dense_check): one per device,
+// sticky, set by a kernel whose bounded wait expired.
+#include "gemm_tc.cuh"
 
 namespace glmx {
 
 static __device__ int g_dense_err;
 
-cudaError_t dense_err_ptr(int** p) { return cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_dense_err); }
+int dense_device()
+{
+    int d = -1;
+    return cudaGetDevice(&d) == cudaSuccess ? d : -1;
+}
+
+cudaError_t dense_err_ptr(int** p)
+{
+    static int* ptr[64] = {};
+    const int d = dense_device();
+    if (d < 0 || d >= 64) return cudaErrorInvalidDevice;
+    if (!ptr[d])
+    {
+        int* q = nullptr;
+        const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&q), g_dense_err);
+        if (e != cudaSuccess) return e;
+        ptr[d] = q;
+    }
+    *p = ptr[d];
+    return cudaSuccess;
+}
+
+int dense_sms(int device)
+{
+    static int n[64] = {};
+    if (!n[device])
+    {
+        int v = 0;
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || v < 2) v = 2;
+        n[device] = v;
+    }
+    return n[device];
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+cudaError_t dense_map(CUtensorMap* m, int dtype, const Mat& t, int box_inner, int box_rows)
+{
+    static EncodeTiledFn fn = nullptr;
+    if (!fn)
+    {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+        if (!fn) return cudaErrorNotSupported;
+    }
+    const bool bytes = dtype != GLMX_F16 && dtype != GLMX_BF16;
+    const cuuint64_t dims[2] = { (cuuint64_t) t.inner, (cuuint64_t) t.rows };
+    const cuuint64_t strides[1] = { (cuuint64_t) t.pitch * (bytes ? 1 : 2) };
+    const cuuint32_t box[2] = { (cuuint32_t) box_inner, (cuuint32_t) box_rows };
+    const cuuint32_t es[2] = { 1, 1 };
+    const CUtensorMapDataType type = bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                           : dtype == GLMX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = fn(m, type, 2, const_cast<void*>(t.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
 
 }  // namespace glmx
 

@@ -1,0 +1,776 @@
+// Matrix products of the dense operators on the 5th-generation tensor cores (tcgen05, accumulators in tensor memory), with
+// their epilogues. Two kernels:
+//
+//   pair_kernel: many rows. Persistent CTA pairs (cta_group::2), 256 tokens x 256 columns per tile, each CTA holding half of the
+//     rows of A and half of the columns of B, so that a byte of shared memory feeds 256 products' worth of either side.
+//   cols_kernel: few rows. The weights are the M operand (128 of their rows per tile), the tokens the N operand (16 .. 256),
+//     and K is split over the CTAs of a cluster, whose partial tiles are added in rank order over distributed shared memory:
+//     enough CTAs to stream the weights at full bandwidth, one launch, no scratch, the same bits in every run.
+//
+// Operands are row-major matrices read by TMA with the 128-byte swizzle: K-major ones [rows][K] in boxes of 128 bytes of K,
+// MN-major ones [K][rows] in boxes of 64 rows x 64 K. Boxes past an edge are zero-filled; stores are predicated.
+#pragma once
+#include <cuda.h>
+
+#include "dense.h"
+#include "glmx_common.cuh"
+
+namespace glmx {
+
+enum { EPI_GATED, EPI_STORE, EPI_DACT, EPI_I8 };
+
+// What becomes of the sums: element (t, n) of an [M tokens][N] result.
+struct Epi
+{
+    int M, N;
+    int bf16;                   // 16-bit type: bf16 or fp16
+    int vec;                    // rows of every output can take 16-byte stores
+    void* y; long long ldy; int y_dtype, accumulate;     // STORE, I8
+    void* o0; void* o1;         // GATED: o0 = h; DACT: o0 = dg, o1 = du, [M][N]
+    float* p; float* q;
+    float limit;
+    const float* xs; const float* ws; const float* bias; // I8
+};
+
+template <int W>
+__device__ __forceinline__ void store16(void* base, size_t off, const float (&v)[W], int bf16)
+{
+    uint32_t w[W / 2];
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i)
+    {
+        if (bf16)
+        {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        else
+        {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    uint8_t* d = static_cast<uint8_t*>(base) + off * 2;
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ float load16(const void* base, size_t off, int bf16)
+{
+    return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[off]) : __half2float(static_cast<const __half*>(base)[off]);
+}
+
+template <int W>
+__device__ __forceinline__ void store_f32(float* d, const float (&v)[W])
+{
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) reinterpret_cast<float4*>(d)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+
+// W (4 or 8) consecutive columns n .. n + W - 1 of token t; n is a multiple of W. v: the sums (GATED: of gate; u of up).
+// I8 sums are int32 bit patterns.
+template <int EPI, int W>
+__device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t (&acc)[W], const uint32_t (&acc2)[W])
+{
+    if (t >= e.M || n >= e.N) return;
+    float v[W];
+    if constexpr (EPI == EPI_GATED)
+    {
+        // N is a multiple of 8: all W columns are inside
+        const size_t o = (size_t) t * e.N + n;
+        const float L = e.limit;
+        float hh[W], pp[W], qq[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+        {
+            const float g = __uint_as_float(acc[i]), u = __uint_as_float(acc2[i]);
+            const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+            // silu(-inf) = 0 (not -inf * 0)
+            float act = g < -100.0f ? 0.0f : g * s, up = u;
+            const bool kg = L == 0.0f || act <= L, ku = L == 0.0f || fabsf(u) <= L;
+            if (L != 0.0f) { act = fminf(act, L); up = fminf(fmaxf(u, -L), L); if (u != u) up = u; if (g != g) act = g; }
+            hh[i] = act * up;
+            pp[i] = ku ? act : 0.0f;
+            qq[i] = kg ? up * (s + (g < -100.0f ? 0.0f : g * s * (1.0f - s))) : 0.0f;
+        }
+        store16<W>(e.o0, o, hh, e.bf16);
+        if (e.p) { store_f32<W>(e.p + o, pp); store_f32<W>(e.q + o, qq); }
+        return;
+    }
+    if constexpr (EPI == EPI_DACT)
+    {
+        const size_t o = (size_t) t * e.N + n;
+        float dg[W], du[W];
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i)
+        {
+            const float4 p = *reinterpret_cast<const float4*>(e.p + o + 4 * i), q = *reinterpret_cast<const float4*>(e.q + o + 4 * i);
+            const float pv[4] = { p.x, p.y, p.z, p.w }, qv[4] = { q.x, q.y, q.z, q.w };
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+            {
+                const float d = __uint_as_float(acc[4 * i + j]);
+                dg[4 * i + j] = d * qv[j];
+                du[4 * i + j] = d * pv[j];
+            }
+        }
+        store16<W>(e.o0, o, dg, e.bf16);
+        store16<W>(e.o1, o, du, e.bf16);
+        return;
+    }
+    if constexpr (EPI == EPI_I8)
+    {
+        const float xs = e.xs[t];
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+        {
+            const int c = n + i < e.N ? n + i : e.N - 1;
+            v[i] = (float) (int) acc[i] * (xs * e.ws[c]);
+            if (e.bias) v[i] += e.bias[c];
+        }
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = __uint_as_float(acc[i]);
+    }
+    const size_t o = (size_t) t * e.ldy + n;
+    const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
+    if (e.vec && n + W <= e.N)
+    {
+        if (e.accumulate)
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] += f32 ? static_cast<const float*>(e.y)[o + i] : load16(e.y, o + i, bf);
+        if (f32) store_f32<W>(static_cast<float*>(e.y) + o, v);
+        else store16<W>(e.y, o, v, bf);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+    {
+        if (n + i >= e.N) break;
+        if (f32)
+        {
+            float* d = static_cast<float*>(e.y) + o + i;
+            *d = e.accumulate ? *d + v[i] : v[i];
+        }
+        else
+        {
+            const float w = e.accumulate ? load16(e.y, o + i, bf) + v[i] : v[i];
+            if (bf) static_cast<__nv_bfloat16*>(e.y)[o + i] = __float2bfloat16_rn(w);
+            else static_cast<__half*>(e.y)[o + i] = __float2half_rn(w);
+        }
+    }
+}
+
+// ---- tcgen05 / TMA / cluster primitives ------------------------------------------------------------------------------
+
+// shared-memory matrix descriptor with the 128-byte swizzle. K-major: 8-row groups 1024 bytes apart (leading offset
+// unused). MN-major: 64-row blocks `lbo` apart, 8-K groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo)
+{
+    return (uint64_t) ((saddr & 0x3FFFFu) >> 4) | ((uint64_t) (lbo >> 4) << 16) | ((uint64_t) (1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+
+// instruction descriptor: 16-bit floats to fp32, or signed bytes to int32; bits 15 / 16 for MN-major A / B
+__host__ __device__ constexpr uint32_t tc_idesc(bool i8, bool bf16, bool a_mn, bool b_mn, int m, int n)
+{
+    return ((i8 ? 2u : 1u) << 4) | ((i8 || bf16 ? 1u : 0u) << 7) | ((i8 || bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) |
+           ((b_mn ? 1u : 0u) << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (m >> 4) << 24);
+}
+
+template <bool I8, int CG>
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc)
+{
+    const uint32_t en = acc;
+    if constexpr (I8 && CG == 1)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(en));
+    else if constexpr (I8)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(en));
+    else if constexpr (CG == 1)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(en));
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(en));
+}
+
+// arrive on `bar` (CG 2: on both CTAs' barrier at that offset) once this thread's earlier MMAs are complete
+template <int CG>
+__device__ __forceinline__ void tc_commit(uint64_t* bar)
+{
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t) 3) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tc_alloc(uint32_t* slot, uint32_t cols)
+{
+    if constexpr (CG == 1)
+    {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    else
+    {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+
+template <int CG>
+__device__ __forceinline__ void tc_dealloc(uint32_t tmem, uint32_t cols)
+{
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+}
+
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 16 consecutive 32-bit columns of this thread's tensor-memory lane (valid after tc_wait_ld)
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// address of rank's copy of a shared-memory address
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// a CTA pair's load: into this CTA's shared memory, counted on a barrier that may be the other CTA's
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// wait for asynchronous copies that nobody will wait for any more (only after a bounded wait has expired)
+__device__ __forceinline__ void drain_pause()
+{
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 1000000) __nanosleep(10000);
+}
+
+// ---- pair_kernel -------------------------------------------------------------------------------------------------------
+
+constexpr int MAXPROB = 3;
+
+struct PairMaps
+{
+    CUtensorMap a[MAXPROB], b[MAXPROB];
+};
+
+struct PairArgs
+{
+    int nprob;                  // products in the launch (the weights' gradients: three); problem p has maps a[p], b[p], epilogue e[p]
+    int nseg;                   // 1; 2: one product whose sum runs over a[0] b[0] and a[1] b[1]
+    int K, bk;                  // inputs per segment, and per stage (128 bytes)
+    int BN;                     // columns per tile: 128 or 256
+    int mt[MAXPROB], nt[MAXPROB], tile0[MAXPROB + 1];    // tiles along M and N, and the first tile of each problem
+    uint32_t idesc;
+    int* err;
+    Epi e[MAXPROB];
+};
+
+constexpr int PAIR_BM = 128;                             // rows per CTA, 256 per pair
+constexpr int PAIR_EPI = 8;                              // epilogue warps: two per tensor-memory lane quarter
+constexpr int PAIR_THREADS = (2 + PAIR_EPI) * 32;
+constexpr int PAIR_STAGES_MAX = 8;
+constexpr int PAIR_SMEM = 227 * 1024;
+constexpr int pair_stage(int bn) { return PAIR_BM * 128 + bn / 2 * 128; }
+constexpr int pair_stages(int bn)
+{
+    const int n = (PAIR_SMEM - 1024 - 2048) / pair_stage(bn);   // 1 KB of static shared memory, 2 KB of alignment
+    return n > PAIR_STAGES_MAX ? PAIR_STAGES_MAX : n;
+}
+constexpr int pair_smem(int bn) { return 2048 + pair_stages(bn) * pair_stage(bn); }
+
+// I8: signed bytes; A_MN / B_MN: operand stored [K][rows]; EPI
+template <bool I8, bool A_MN, bool B_MN, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairArgs a)
+{
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[PAIR_STAGES_MAX], empty[PAIR_STAGES_MAX], tfull[2], tempty[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int s_abort;
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int BN = a.BN, NST = pair_stages(BN), STAGE = pair_stage(BN);
+    if (tid == 0)
+    {
+        for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&tfull[s], 1); mbar_init(&tempty[s], 2 * PAIR_EPI); }
+        s_abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tc_alloc<2>(&tmem_slot, 512);
+    tc_before();
+    __syncthreads();
+    cluster_sync();
+    tc_after();
+    const uint32_t tmem = tmem_slot;
+    grid_release();
+    grid_wait();
+
+    const int pairs = gridDim.x >> 1, first = blockIdx.x >> 1, ntiles = a.tile0[a.nprob];
+    const int ksteps = (a.K + a.bk - 1) / a.bk, nk = ksteps * a.nseg;
+    auto find = [&](int t, int& p, int& m, int& n) {
+        p = 0;
+        while (p + 1 < a.nprob && t >= a.tile0[p + 1]) ++p;
+        t -= a.tile0[p];
+        m = t % a.mt[p];
+        n = t / a.mt[p];
+    };
+
+    if (warp == 0)
+    {
+        if (lane == 0)
+        {
+            int it = 0;
+            for (int t = first; t < ntiles && !s_abort; t += pairs)
+            {
+                int p, m, n;
+                find(t, p, m, n);
+                for (int k = 0; k < nk; ++k, ++it)
+                {
+                    const int s = it % NST;
+                    if (!mbar_wait_bounded(&empty[s], (uint32_t) ((it / NST) & 1) ^ 1u)) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
+                    const int seg = k / ksteps, kc = (k - seg * ksteps) * a.bk, mp = a.nseg > 1 ? seg : p;
+                    uint8_t* sa = smem + (size_t) s * STAGE;
+                    uint8_t* sb = sa + PAIR_BM * 128;
+                    // the pair's four half tiles are counted on the leader's barrier
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t) (2 * STAGE));
+                    const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
+                    const int m0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM;
+                    if constexpr (A_MN)
+                        for (int j = 0; j < 2; ++j) tma_load_pair(sa + j * 8192, &maps.a[mp], m0 + 64 * j, kc, bar);
+                    else
+                        tma_load_pair(sa, &maps.a[mp], kc, m0, bar);
+                    if constexpr (EPI == EPI_GATED)
+                        // gate columns from CTA 0, the same up columns from CTA 1
+                        tma_load_pair(sb, &maps.b[rank], kc, n * (BN / 2), bar);
+                    else
+                    {
+                        const int n0 = n * BN + (int) rank * (BN / 2);
+                        if constexpr (B_MN)
+                            for (int j = 0; j < BN / 128; ++j) tma_load_pair(sb + j * 8192, &maps.b[mp], n0 + 64 * j, kc, bar);
+                        else
+                            tma_load_pair(sb, &maps.b[mp], kc, n0, bar);
+                    }
+                }
+            }
+            // the last arrivals on this CTA's barriers come from the pair's leader: they are in before it may exit
+            for (int i = it > NST ? it - NST : 0; i < it && !s_abort; ++i)
+                if (!mbar_wait_bounded(&empty[i % NST], (uint32_t) ((i / NST) & 1))) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; }
+        }
+    }
+    else if (warp == 1)
+    {
+        if (lane == 0 && rank == 0)
+        {
+            int it = 0, lt = 0;
+            for (int t = first; t < ntiles && !s_abort; t += pairs, ++lt)
+            {
+                const int acc = lt & 1;
+                if (!mbar_wait_bounded(&tempty[acc], (uint32_t) ((lt >> 1) & 1) ^ 1u)) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
+                tc_after();
+                for (int k = 0; k < nk; ++k, ++it)
+                {
+                    const int s = it % NST;
+                    if (!mbar_wait_bounded(&full[s], (uint32_t) ((it / NST) & 1))) { atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
+                    tc_after();
+                    const uint32_t sa = smem_u32(smem + (size_t) s * STAGE), sb = sa + PAIR_BM * 128;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        tc_mma<I8, 2>(tmem + (uint32_t) (acc * 256), desc_sw128(sa + kk * (A_MN ? 2048 : 32), 8192),
+                                      desc_sw128(sb + kk * (B_MN ? 2048 : 32), 8192), a.idesc, (k | kk) != 0);
+                    tc_commit<2>(&empty[s]);
+                }
+                if (s_abort) break;
+                tc_commit<2>(&tfull[acc]);
+            }
+        }
+    }
+    else
+    {
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        int lt = 0;
+        for (int t = first; t < ntiles && !s_abort; t += pairs, ++lt)
+        {
+            const int acc = lt & 1;
+            int p, m, n;
+            find(t, p, m, n);
+            if (!mbar_wait_bounded(&tfull[acc], (uint32_t) ((lt >> 1) & 1))) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
+            tc_after();
+            const Epi& e = a.e[p];
+            const int row = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q + lane;
+            const uint32_t tq = tmem + ((uint32_t) (32 * q) << 16) + (uint32_t) (acc * 256);
+            // this warp's half of the tile's columns, 16 at a time
+            const int cols = EPI == EPI_GATED ? BN / 4 : BN / 2, c0 = half * cols;
+            for (int c = c0; c < c0 + cols; c += 16)
+            {
+                uint32_t v[16], u[16];
+                tc_ld16(tq + (uint32_t) c, v);
+                if constexpr (EPI == EPI_GATED) tc_ld16(tq + (uint32_t) (BN / 2 + c), u);
+                tc_wait_ld();
+                const int nn = n * (EPI == EPI_GATED ? BN / 2 : BN) + c;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                {
+                    uint32_t v8[8], u8[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { v8[i] = v[8 * j + i]; u8[i] = EPI == EPI_GATED ? u[8 * j + i] : 0; }
+                    emit<EPI, 8>(e, row, nn + 8 * j, v8, u8);
+                }
+            }
+            tc_before();
+            __syncwarp();
+            if (lane == 0) arrive_remote(map_rank(smem_u32(&tempty[acc]), 0));
+        }
+    }
+    __syncwarp();
+    if (s_abort) drain_pause();
+    tc_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1)
+    {
+        tc_after();
+        tc_dealloc<2>(tmem, 512);
+    }
+}
+
+// ---- cols_kernel -------------------------------------------------------------------------------------------------------
+
+struct ColsMaps
+{
+    CUtensorMap w[2], x[2];     // weights (GATED: gate, up; two segments: one each) and tokens
+};
+
+struct ColsArgs
+{
+    int nseg, K, bk;
+    int NT;                     // tokens per tile: a multiple of 16, at most 256
+    int stages;
+    int mtiles;                 // weight-row tiles; the grid is [splits][mtiles * token tiles]
+    int tcols;                  // tensor-memory columns: a power of 2 >= NT, at least 32
+    int prefetch;               // weights may be read before the kernels in front have finished
+    uint32_t idesc;
+    int* err;
+    Epi e;
+};
+
+constexpr int COLS_THREADS = 192;
+constexpr int COLS_STAGES_MAX = 12;
+
+template <bool I8, bool W_MN, int EPI>
+__global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_constant__ ColsMaps maps, const __grid_constant__ ColsArgs a)
+{
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[COLS_STAGES_MAX], empty[COLS_STAGES_MAX], tfull;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int s_abort;
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int splits = gridDim.x, split = blockIdx.x;      // one cluster along x
+    const int mtile = blockIdx.y % a.mtiles, ttile = blockIdx.y / a.mtiles;
+    const int NT = a.NT, NST = a.stages, STAGE = 16384 + NT * 128;
+    if (tid == 0)
+    {
+        for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(&tfull, 1);
+        s_abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tc_alloc<1>(&tmem_slot, (uint32_t) a.tcols);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_slot;
+    grid_release();
+
+    const int ksteps = (a.K + a.bk - 1) / a.bk, nk_all = ksteps * a.nseg;
+    const int k0 = (int) ((long long) nk_all * split / splits), nk = (int) ((long long) nk_all * (split + 1) / splits) - k0;
+    const int rows = EPI == EPI_GATED ? 64 : 128;          // output columns (weight rows of one matrix) per tile
+
+    if (warp == 0)
+    {
+        if (lane == 0)
+        {
+            auto load_w = [&](int i) {
+                const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
+                uint8_t* sw = smem + (size_t) s * STAGE;
+                mbar_arrive_expect_tx(&full[s], (uint32_t) STAGE);
+                if constexpr (EPI == EPI_GATED)
+                    for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[j], kc, mtile * 64, &full[s]);
+                else if constexpr (W_MN)
+                    for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[seg], mtile * 128 + 64 * j, kc, &full[s]);
+                else
+                    tma_load_2d(sw, &maps.w[seg], kc, mtile * 128, &full[s]);
+            };
+            auto load_x = [&](int i) {
+                const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
+                tma_load_2d(smem + (size_t) s * STAGE + 16384, &maps.x[seg], kc, ttile * NT, &full[s]);
+            };
+            const int ahead = a.prefetch ? (nk < NST ? nk : NST) : 0;
+            for (int i = 0; i < ahead; ++i) load_w(i);
+            grid_wait();
+            for (int i = 0; i < ahead; ++i) load_x(i);
+            for (int i = ahead; i < nk; ++i)
+            {
+                const int s = i % NST;
+                if (!mbar_wait_bounded(&empty[s], (uint32_t) ((i / NST) & 1) ^ 1u)) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
+                load_w(i);
+                load_x(i);
+            }
+        }
+    }
+    else if (warp == 1)
+    {
+        grid_wait();
+        if (lane == 0)
+        {
+            for (int i = 0; i < nk; ++i)
+            {
+                const int s = i % NST;
+                if (!mbar_wait_bounded(&full[s], (uint32_t) ((i / NST) & 1))) { atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
+                tc_after();
+                const uint32_t sw = smem_u32(smem + (size_t) s * STAGE), sx = sw + 16384;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    tc_mma<I8, 1>(tmem, desc_sw128(sw + kk * (W_MN ? 2048 : 32), 8192), desc_sw128(sx + kk * 32, 8192), a.idesc, (i | kk) != 0);
+                tc_commit<1>(&empty[s]);
+            }
+            tc_commit<1>(&tfull);
+        }
+    }
+    __syncwarp();
+    grid_wait();
+    // every load has been multiplied: the partial tile [token][weight row] takes the ring's place
+    if (!mbar_wait_bounded(&tfull, 0)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; }
+    if (s_abort) drain_pause();
+    __syncthreads();
+    tc_after();
+    float* part = reinterpret_cast<float*>(smem);
+    const int ncols = min(NT, a.e.M - ttile * NT);         // tokens of the tile that exist
+    if (warp >= 2 && !s_abort)
+    {
+        const int q = warp & 3;
+        const uint32_t tq = tmem + ((uint32_t) (32 * q) << 16);
+        for (int c = 0; c < ncols; c += 16)
+        {
+            uint32_t v[16];
+            tc_ld16(tq + (uint32_t) c, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) part[(c + i) * 128 + 32 * q + lane] = __uint_as_float(v[i]);
+        }
+    }
+    tc_before();
+    if (splits > 1) cluster_sync(); else __syncthreads();
+    if (warp == 1)
+    {
+        tc_after();
+        tc_dealloc<1>(tmem, (uint32_t) a.tcols);
+    }
+    // groups of 4 weight rows of one token, spread over the cluster's CTAs; partials are added in rank order
+    const int per = rows / 4, units = ncols * per;
+    const int u0 = (int) ((long long) units * split / splits), u1 = (int) ((long long) units * (split + 1) / splits);
+    const uint32_t base = smem_u32(part);
+    if (!s_abort)
+        for (int u = u0 + tid; u < u1; u += COLS_THREADS)
+        {
+            const int c = u / per, r = (u - c * per) * 4;
+            uint32_t v[4] = {}, w[4] = {};
+            auto add = [&](uint32_t (&d)[4], uint32_t off, int rk) {
+                uint32_t x[4];
+                asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(map_rank(base + off, (uint32_t) rk)) : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = rk == 0 ? x[i] : I8 ? d[i] + x[i] : __float_as_uint(__fadd_rn(__uint_as_float(d[i]), __uint_as_float(x[i])));
+            };
+            for (int rk = 0; rk < splits; ++rk)
+            {
+                add(v, (uint32_t) (c * 128 + r) * 4, rk);
+                if constexpr (EPI == EPI_GATED) add(w, (uint32_t) (c * 128 + 64 + r) * 4, rk);
+            }
+            emit<EPI, 4>(a.e, ttile * NT + c, mtile * rows + r, v, w);
+        }
+    __syncwarp();
+    if (splits > 1) cluster_sync();                        // nobody leaves while its partial tile is read
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+
+// a row-major matrix operand: [rows][inner], rows `pitch` elements apart
+struct Mat
+{
+    const void* p;
+    long long rows, inner, pitch;
+};
+
+// tensor map of boxes of box_inner x box_rows elements with the 128-byte swizzle
+cudaError_t dense_map(CUtensorMap* m, int dtype, const Mat& t, int box_inner, int box_rows);
+cudaError_t dense_err_ptr(int** p);          // the current device's error word
+int dense_device();                          // the current device, or -1
+int dense_sms(int device);
+
+// One product of the launch: sums over segs (A: tokens, B: weights; GATED: B of seg 0 and 1 are gate and up)
+struct Product
+{
+    Mat a[2], b[2];
+    Epi e;
+};
+
+template <bool I8, bool A_MN, bool B_MN, int EPI>
+cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K, int BN, cudaStream_t st)
+{
+    auto kernel = pair_kernel<I8, A_MN, B_MN, EPI>;
+    const int dev = dense_device();
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    static bool ready[64] = {};
+    cudaError_t err;
+    if (!ready[dev])
+    {
+        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM - 1024)) != cudaSuccess) return err;
+        ready[dev] = true;
+    }
+    PairMaps maps;
+    PairArgs a{};
+    a.nprob = nprob; a.nseg = nseg; a.K = K; a.bk = I8 ? 128 : 64; a.BN = BN;
+    a.idesc = tc_idesc(I8, dtype == GLMX_BF16, A_MN, B_MN, 256, BN);
+    if ((err = dense_err_ptr(&a.err)) != cudaSuccess) return err;
+    const int width = EPI == EPI_GATED ? BN / 2 : BN;
+    for (int i = 0; i < nprob; ++i)
+    {
+        a.e[i] = pr[i].e;
+        a.mt[i] = (pr[i].e.M + 255) / 256;
+        a.nt[i] = (pr[i].e.N + width - 1) / width;
+        a.tile0[i + 1] = a.tile0[i] + a.mt[i] * a.nt[i];
+    }
+    for (int i = 0; i < (nprob > 1 ? nprob : nseg); ++i)
+    {
+        const Mat& ma = nprob > 1 ? pr[i].a[0] : pr[0].a[i];
+        if ((err = dense_map(&maps.a[i], dtype, ma, A_MN ? 64 : a.bk, A_MN ? 64 : PAIR_BM)) != cudaSuccess) return err;
+    }
+    for (int i = 0; i < (EPI == EPI_GATED ? 2 : nprob > 1 ? nprob : nseg); ++i)
+    {
+        const Mat& mb = nprob > 1 ? pr[i].b[0] : pr[0].b[i];
+        if ((err = dense_map(&maps.b[i], dtype, mb, B_MN ? 64 : a.bk, B_MN ? 64 : BN / 2)) != cudaSuccess) return err;
+    }
+    const int tiles = a.tile0[nprob], pairs = dense_sms(dev) / 2;
+    return launch_chained(kernel, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), (size_t) pair_smem(BN), st, maps, a);
+}
+
+struct ColsPlan
+{
+    int NT, ttiles, mtiles, splits, stages;
+};
+
+// Tokens per tile: all of them up to 256, else equal tiles. Splits of K: the count (at most 8, the portable cluster size) that
+// leaves the SMs the fewest rounds of the least work, each CTA with at least two stages.
+inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms)
+{
+    ColsPlan p;
+    p.ttiles = (M + 255) / 256;
+    p.NT = ((M + p.ttiles - 1) / p.ttiles + 15) / 16 * 16;
+    p.mtiles = (N + (gated ? 63 : 127)) / (gated ? 64 : 128);
+    const int stage = 16384 + p.NT * 128, tiles = p.ttiles * p.mtiles;
+    p.splits = 1;
+    double best = 1e30;
+    for (int s = 1; s <= 8 && (s == 1 || 2 * s <= nk); ++s)
+    {
+        const double rounds = (double) ((tiles * s + sms - 1) / sms), cost = rounds * ((nk + s - 1) / s + 2.0);
+        if (cost < best - 1e-9) { best = cost; p.splits = s; }
+    }
+    const int room = p.NT <= 64 ? 112 * 1024 : 224 * 1024, per = (nk + p.splits - 1) / p.splits;
+    p.stages = (room - 2048) / stage;
+    if (p.stages > COLS_STAGES_MAX) p.stages = COLS_STAGES_MAX;
+    const int part = (p.NT * 512 + stage - 1) / stage;     // the partial tile takes the ring's place
+    if (p.stages > per) p.stages = per;
+    if (p.stages < part) p.stages = part;
+    return p;
+}
+
+template <bool I8, bool W_MN, int EPI>
+cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, bool prefetch, cudaStream_t st)
+{
+    auto kernel = cols_kernel<I8, W_MN, EPI>;
+    const int dev = dense_device();
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    static bool ready[64] = {};
+    cudaError_t err;
+    if (!ready[dev])
+    {
+        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024)) != cudaSuccess) return err;
+        ready[dev] = true;
+    }
+    ColsMaps maps;
+    ColsArgs a{};
+    a.nseg = nseg; a.K = K; a.bk = I8 ? 128 : 64;
+    const ColsPlan p = cols_plan(pr.e.M, pr.e.N, EPI == EPI_GATED, nseg * ((K + a.bk - 1) / a.bk), dense_sms(dev));
+    a.NT = p.NT; a.stages = p.stages; a.mtiles = p.mtiles; a.prefetch = prefetch;
+    a.tcols = 32;
+    while (a.tcols < p.NT) a.tcols *= 2;
+    a.idesc = tc_idesc(I8, dtype == GLMX_BF16, W_MN, false, 128, p.NT);
+    if ((err = dense_err_ptr(&a.err)) != cudaSuccess) return err;
+    a.e = pr.e;
+    for (int i = 0; i < (EPI == EPI_GATED ? 2 : nseg); ++i)
+        if ((err = dense_map(&maps.w[i], dtype, pr.b[i], W_MN ? 64 : a.bk, W_MN || EPI == EPI_GATED ? 64 : 128)) != cudaSuccess) return err;
+    for (int i = 0; i < nseg; ++i)
+        if ((err = dense_map(&maps.x[i], dtype, pr.a[i], a.bk, p.NT)) != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits, p.mtiles * p.ttiles);
+    cfg.blockDim = dim3(COLS_THREADS);
+    cfg.dynamicSmemBytes = 1024 + (size_t) p.stages * (16384 + p.NT * 128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, maps, a);
+}
+
+// Which kernel: few rows go to cols_kernel, many to pair_kernel. Measured (us, cols / pair): feed-forward of 256 rows at
+// H = 6144, I = 1536 62 / 63 and of 512 rows 91 / 64; int8 product of 48 rows at K = N = 6144 13 / 31, of 256 rows 40 / 33.
+inline bool use_pair(int M, bool i8) { return M > (i8 ? 160 : 384); }
+
+}  // namespace glmx

@@ -1,6 +1,6 @@
 // 8-bit linear (glmx_quantize_rows, glmx_linear_i8): rows to int8 with one scale each, and the product of two int8
-// matrices with a scale per token and per output channel. Simple form of the product: dp4a on the CUDA cores.
-#include "dense.h"
+// matrices with a scale per token and per output channel.
+#include "gemm_tc.cuh"
 
 namespace glmx {
 
@@ -31,54 +31,6 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* x, long long ldx
     signed char* qr = q + (size_t) blockIdx.x * ldq;
     for (int k = threadIdx.x; k < K; k += 256)
         qr[k] = (signed char) (s > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(to_f32(xr[k]), s)))) : 0);
-}
-
-struct I8Args
-{
-    const signed char* x; long long ldx; const float* xs;
-    const signed char* w; long long ldw; const float* ws;
-    const float* bias;
-    void* y; long long ldy; int y_dtype;
-    int M, N, K;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) i8_simple_kernel(I8Args a)
-{
-    constexpr int TS = 64, TW = 16;                        // 64 x 64 outputs, 16 words of 4 inputs per step
-    __shared__ int sa[TW][TS + 1], sb[TW][TS + 1];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, m0 = blockIdx.y * TS, n0 = blockIdx.x * TS;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += 4 * TW)
-    {
-        for (int i = threadIdx.x; i < TS * TW; i += 256)
-        {
-            const int r = i / TW, w = i % TW;
-            uint32_t va = 0, vb = 0;
-            for (int c = 0; c < 4; ++c)
-            {
-                const int k = k0 + 4 * w + c;
-                if (k < a.K && m0 + r < a.M) va |= (uint32_t) (uint8_t) a.x[(m0 + r) * a.ldx + k] << (8 * c);
-                if (k < a.K && n0 + r < a.N) vb |= (uint32_t) (uint8_t) a.w[(n0 + r) * a.ldw + k] << (8 * c);
-            }
-            sa[w][r] = (int) va;
-            sb[w][r] = (int) vb;
-        }
-        __syncthreads();
-        for (int w = 0; w < TW; ++w)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sa[w][ty * 4 + i], sb[w][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j)
-        {
-            const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= a.M || n >= a.N) continue;
-            float v = (float) acc[i][j] * (a.xs[m] * a.ws[n]);
-            if (a.bias) v += a.bias[n];
-            static_cast<T*>(a.y)[m * a.ldy + n] = from_f32<T>(v);
-        }
 }
 
 }  // namespace
@@ -117,11 +69,13 @@ extern "C" int glmx_linear_i8(const signed char* xq, long long ldxq, const float
     if (!xq || !x_scale || !wq || !w_scale || !y) return dense_fail(GLMX_E_ARG, "glmx_linear_i8: null argument");
     if (!dense_aligned(xq) || !dense_aligned(wq)) return dense_fail(GLMX_E_ARG, "glmx_linear_i8: xq and wq must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const I8Args a{ xq, ldxq, x_scale, wq, ldwq, w_scale, bias, y, ldy, y_dtype, ntok, N, K };
-    const dim3 grid((N + 63) / 64, (ntok + 63) / 64);
-    if (y_dtype == GLMX_F32) i8_simple_kernel<float><<<grid, 256, 0, st>>>(a);
-    else if (y_dtype == GLMX_F16) i8_simple_kernel<__half><<<grid, 256, 0, st>>>(a);
-    else i8_simple_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    Product p{};
+    p.a[0] = { xq, ntok, K, ldxq };
+    p.b[0] = { wq, N, K, ldwq };
+    p.e.M = ntok; p.e.N = N; p.e.y = y; p.e.ldy = ldy; p.e.y_dtype = y_dtype;
+    p.e.xs = x_scale; p.e.ws = w_scale; p.e.bias = bias;
+    p.e.vec = dense_aligned(y) && ldy * (y_dtype == GLMX_F32 ? 4 : 2) % 16 == 0;
+    const cudaError_t e = use_pair(ntok, true) ? launch_pair<true, false, false, EPI_I8>(GLMX_I32, 1, &p, 1, K, 256, st)
+                                                        : launch_cols<true, false, EPI_I8>(GLMX_I32, p, 1, K, false, st);
     return e == cudaSuccess ? GLMX_OK : dense_cuda_fail(e, "glmx_linear_i8: launch");
 }
