@@ -3,13 +3,15 @@
 // block scans), a batch by the exponentials of the rows that keep many tokens.
 //
 // A weight is w = exp((l - m) / T) <= 1 in fp32, held as the integer floor(w * 2^44): sums of up to 2^19 weights fit 64 bits
-// and do not depend on their order. Equal logits have equal weights, so each filter is a threshold on the logits'
-// order-preserving integer key plus a number of kept ties, the lowest ids first:
-//   top-k: the key with count(>) < k <= count(>=);  top-p: the key with mass(>) < top_p * S <= mass(>=);  min-p: a least weight.
-// The first histogram (1024 bins of m - l, as wide as 2^-44 reaches) finds the bin in which the first active filter ends. Where
-// the bins up to it hold at most 512 logits, these are gathered and sorted in one CTA, which finishes the row. Otherwise the
-// threshold is narrowed by further histograms of 1024 bins over the keys of that bin, and the pick is found by
-// running sums over the row: the CTA, the warp, then the lane in whose run the target falls.
+// and do not depend on their order. Equal logits have equal weights, so each filter is a threshold on the logits plus a
+// number of kept ties, the lowest ids first:
+//   top-k: the value with count(>) < k <= count(>=);  top-p: the value with mass(>) < top_p * S <= mass(>=);  min-p: a least weight.
+// Few logits matter as a rule. The largest logit of each thread's share is known from the load: where k of these lie above a bin's
+// edge, the top k logits do. What lies above is gathered (at most 512 logits, else the general way) and sorted in one
+// CTA, which finishes the row; without a top-k the same is done where the gathered weights reach top_p.
+// Otherwise the threshold is found by a histogram of 1024 bins of m - l, narrowed by histograms over the keys
+// (order-preserving integers) of one bin, and the pick by running sums over the row: the CTA, the warp, then the lane in
+// whose run the target falls.
 #include "dense.h"
 #include "glmx_common.cuh"
 
@@ -29,7 +31,8 @@ struct SampleArgs
 
 constexpr int ST = 512, SBINS = 1024, SLIST = 512, SRANKS = 8;
 constexpr int SLICE_MAX = GLMX_SAMPLE_MAX_VOCAB / SRANKS;  // 49152 logits: 192 KB
-constexpr float SPAN = 30.6f;                              // exp(-30.5) = 2^-44: weights further down are 0
+constexpr float SPAN = 16.0f;                              // the first histogram's bins reach down to exp(-16); the last holds the rest
+constexpr int TRY = 320;                                   // without a top-k: thread maxima above the gathered logits' edge
 
 // order-preserving key of a logit that is not NaN; TS bits are the same in all values of the type
 template <typename T> struct KeyShift { static constexpr int v = 0; };
@@ -42,56 +45,57 @@ __device__ __forceinline__ uint32_t key_of(float l)
     return (b & 0x80000000u ? ~b : b | 0x80000000u) >> KeyShift<T>::v;
 }
 
+// the logit of a key: the dropped bits are 0, in negative ones 1
+template <typename T>
+__device__ __forceinline__ float of_key(uint32_t k)
+{
+    const uint32_t full = k << KeyShift<T>::v;
+    return __uint_as_float(full & 0x80000000u ? full & 0x7fffffffu : ~(full | ((1u << KeyShift<T>::v) - 1)));
+}
+
 struct Weight
 {
-    float m, ch, cl;                                       // row maximum, log2(e) / T as hi + lo
+    float m, c;                                            // row maximum, log2(e) / T
     __device__ __forceinline__ void init(float max, float T)
     {
         m = max;
-        const double c = 1.4426950408889634 / (double) T;
-        ch = (float) fmin(c, 3e38);
-        cl = c < 3e38 ? (float) (c - (double) ch) : 0.0f;
+        c = (float) fmin(1.4426950408889634 / (double) T, 3e38);
     }
-    // floor(2^44 exp((l - m) / T)): l - m with its rounding error (two-sum), scaled to a power of 2 in hi + lo, the power
-    // split into an integer and |f| <= 1/2, 2^f by its Taylor series in f ln 2 (0.347^8 / 8! = 5e-9)
+    // floor(2^44 2^((l - m) c)). The exponent's rounding moves a weight of 2^-x by x 2^-24 of itself, the exponential by about 2^-22: no more than
+    // fp32 logits carry. -inf gives 0
     __device__ __forceinline__ u64 operator()(float l) const
     {
-        if (l == m) return 1ull << 44;
-        const float d = l - m, bb = d - l, derr = (l - (d - bb)) + (-m - bb);
-        const float x = d * ch;
-        if (!(x > -46.0f)) return 0;
-        const float lo = fmaf(d, ch, -x) + fmaf(d, cl, derr * ch);
-        const float n = rintf(x), f = ((x - n) + lo) * 0.693147180559945f;
-        float e = fmaf(f, 1.0f / 5040, 1.0f / 720);
-        e = fmaf(e, f, 1.0f / 120); e = fmaf(e, f, 1.0f / 24); e = fmaf(e, f, 1.0f / 6); e = fmaf(e, f, 0.5f);
-        e = fmaf(e, f, 1.0f); e = fmaf(e, f, 1.0f);
-        const u64 w = (u64) __float2uint_rd(e * 16777216.0f);
-        const int sh = 20 + (int) n;
-        return sh >= 0 ? w << sh : w >> -sh;
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((l - m) * c));
+        return __float2ull_rd(e * 17592186044416.0f);
     }
 };
 
 struct Hist
 {
-    uint32_t cnt[SBINS], lo[SBINS], hi[SBINS];             // counts, and 64-bit masses in two words
+    uint32_t lo[4][SBINS], hi[SBINS], cnt[SBINS];          // masses in two words (or counts in the low one), counts. Four copies of
+                                                           // the low word: lanes that hit one bin meet less often
 };
 
 struct Found                                               // the bin in which a running sum reaches its need
 {
-    int bin;
+    int bin;                                               // -1: nowhere
     u64 above, in;                                         // the sum above it and its own
-    uint32_t cnt_above, cnt_in;
+    uint32_t cnt_in;
 };
 
 struct Shared
 {
-    Hist hist[2];
-    u64 mail[2][2][SRANKS];
+    u64 mail[2][3][SRANKS];
     u64 warp[ST / 32];
     uint32_t warp32[ST / 32];
-    u64 list[SLIST];                                       // (key, ~id) of this CTA's gathered logits
-    u64 sorted[SLIST];
-    uint32_t order[SLIST];
+    u64 list[SLIST];                                       // (logit, id) of the gathered logits, in CTA 0
+    uint32_t maxima[SBINS];                                // histogram of the threads' maxima
+    union
+    {
+        Hist hist;
+        struct { u64 sorted[SLIST]; uint32_t order[SLIST]; };
+    };
     Found found;
     int n_list, id;
 };
@@ -107,6 +111,18 @@ __device__ __forceinline__ u64 dsmem_ld(const void* p, uint32_t rank)
     u64 v;
     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(dsmem_map(p, rank)) : "memory");
     return v;
+}
+// the pair of words at p in each of nc CTAs, all loads in flight at once
+__device__ __forceinline__ void dsmem_ld_all(const void* p, int nc, u64 (&v)[SRANKS])
+{
+#pragma unroll
+    for (int r = 0; r < SRANKS; ++r) v[r] = r < nc ? dsmem_ld(p, r) : 0ull;
+}
+__device__ __forceinline__ uint32_t dsmem_add(const void* p, uint32_t rank, uint32_t v)
+{
+    uint32_t old;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(dsmem_map(p, rank)), "r"(v) : "memory");
+    return old;
 }
 __device__ __forceinline__ void dsmem_st(const void* p, uint32_t rank, u64 v)
 {
@@ -146,27 +162,41 @@ __device__ __forceinline__ V block_scan(V v, V* s, V& all)
     return before + v;
 }
 
-// sorts n <= N keys (N a power of 2 from 32 to ST, one a thread) in descending order
-template <typename V>
-__device__ __forceinline__ V block_sort(V v, int N, V* s)
+// sorts N keys, one a thread of threads 0 .. N - 1, in descending order: a bitonic network, exchanges within a warp by shuffles
+template <int N, typename V>
+__device__ __forceinline__ V block_sort(V v, V* s)
 {
     const int t = threadIdx.x;
+#pragma unroll
     for (int size = 2; size <= N; size <<= 1)
+#pragma unroll
         for (int st = size >> 1; st > 0; st >>= 1)
         {
             V o;
             if (st >= 32)
             {
-                __syncthreads();
+                asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
                 s[t] = v;
-                __syncthreads();
+                asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
                 o = s[t ^ st];
             }
             else
                 o = __shfl_xor_sync(0xffffffffu, v, st);
             const bool larger = ((t & st) == 0) == ((t & size) == 0);
-            v = larger ? (v > o ? v : o) : (v < o ? v : o);
+            v = larger == (v > o) ? v : o;
         }
+    return v;
+}
+
+// the same for n <= ST keys; threads from n on bring 0, which no key is
+template <typename V>
+__device__ __forceinline__ V sort_n(V v, int n, V* s)
+{
+    const int t = threadIdx.x;
+    if (n <= 64) { if (t < 64) v = block_sort<64>(v, s); }
+    else if (n <= 128) { if (t < 128) v = block_sort<128>(v, s); }
+    else if (n <= 256) { if (t < 256) v = block_sort<256>(v, s); }
+    else v = block_sort<ST>(v, s);
     return v;
 }
 
@@ -179,22 +209,23 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int NC = gridDim.x, b = blockIdx.y;
     const uint32_t rank = blockIdx.x;
-    const float NONE = __int_as_float(0xff800000);         // -inf: never picked; NaN and what is outside the slice become it
-    int slot = 0, hslot = 0;
+    const float INF = __int_as_float(0x7f800000), NONE = -INF;   // NONE: never picked; NaN and what is outside the slice become it
+    int slot = 0;
     asm volatile("barrier.cluster.arrive.relaxed.aligned;");
 
     auto sync = [&]() {
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     };
-    // every CTA's pair of values, by rank, in sh.mail[the returned slot] (valid until the next exchange but one)
-    auto exchange = [&](u64 v0, u64 v1) {
+    // every CTA's values, by rank, in sh.mail[the returned slot] (valid until the next exchange but one)
+    auto exchange = [&](u64 v0, u64 v1 = 0, u64 v2 = 0) {
         const int sl = slot;
         slot ^= 1;
         if (tid < NC)
         {
             dsmem_st(&sh.mail[sl][0][rank], tid, v0);
             dsmem_st(&sh.mail[sl][1][rank], tid, v1);
+            dsmem_st(&sh.mail[sl][2][rank], tid, v2);
         }
         sync();
         return sl;
@@ -203,42 +234,58 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         if (a.ids64) static_cast<long long*>(a.ids)[b] = id; else static_cast<int*>(a.ids)[b] = id;
     };
 
-    // the slice [s0, s1) of the row into shared memory, in 16-byte loads of whole groups; lg[0] is logit g0, the first of the
-    // aligned group that holds s0
+    // the slice [s0, s1) of the row into shared memory, in 16-byte loads of whole groups, four in flight; lg[0] is logit g0, the
+    // first of the aligned group that holds s0
     constexpr int G = 16 / sizeof(T);
     const T* row = static_cast<const T*>(a.logits) + (size_t) b * a.ld;
     const int s0 = min(a.V, (int) rank * a.per), s1 = min(a.V, s0 + a.per);
     const int head = (int) ((reinterpret_cast<uintptr_t>(row + s0) & 15) / sizeof(T));
     const int g0 = s0 - head, n = (s1 - g0 + G - 1) / G * G * (s1 > s0);
-    float mx = NONE, mn = __int_as_float(0x7f800000);
-    for (int j = tid * G; j < n; j += ST * G)
-    {
-        const int i = g0 + j;
+    float mine_max = NONE;
+    auto take = [&](int j, const float (&v0)[G]) {
         float v[G];
-        if (i >= s0 && i + G <= s1)
-        {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(row + i));
-            const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-            for (int q = 0; q < G; ++q) v[q] = to_f32(e[q]);
-        }
-        else
-        {
-#pragma unroll
-            for (int q = 0; q < G; ++q) v[q] = i + q >= s0 && i + q < s1 ? to_f32(row[i + q]) : NONE;
-        }
 #pragma unroll
         for (int q = 0; q < G; ++q)
         {
-            v[q] = v[q] == v[q] ? v[q] + 0.0f : NONE;      // -0 counts as +0
-            mx = fmaxf(mx, v[q]);
-            if (v[q] != NONE) mn = fminf(mn, v[q]);
+            v[q] = v0[q] == v0[q] ? v0[q] + 0.0f : NONE;   // -0 counts as +0
+            mine_max = fmaxf(mine_max, v[q]);
         }
 #pragma unroll
         for (int q = 0; q < G / 4; ++q) reinterpret_cast<float4*>(lg + j)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    }
+    };
+    for (int jj = tid * G; jj < n; jj += 4 * ST * G)
     {
-        // maximum and minimum over the block, then the cluster
+        uint4 w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            const int j = jj + r * ST * G, i = g0 + j;
+            if (j < n && i >= s0 && i + G <= s1) w[r] = __ldcs(reinterpret_cast<const uint4*>(row + i));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            const int j = jj + r * ST * G, i = g0 + j;
+            if (j >= n) break;
+            float v[G];
+            if (i >= s0 && i + G <= s1)
+            {
+                const T* e = reinterpret_cast<const T*>(&w[r]);
+#pragma unroll
+                for (int q = 0; q < G; ++q) v[q] = to_f32(e[q]);
+            }
+            else
+            {
+#pragma unroll
+                for (int q = 0; q < G; ++q) v[q] = i + q >= s0 && i + q < s1 ? to_f32(row[i + q]) : NONE;
+            }
+            take(j, v);
+        }
+    }
+    for (int i = tid; i < SBINS; i += ST) sh.maxima[i] = 0;
+    // the largest logit, and the smallest of the threads' largest ones
+    float mx = mine_max, mn = mine_max == NONE ? INF : mine_max;
+    {
         for (int o = 16; o; o >>= 1)
         {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -246,6 +293,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         }
         if (lane == 0) { sh.warp32[warp] = __float_as_uint(mx); sh.warp[warp] = __float_as_uint(mn); }
         __syncthreads();
+#pragma unroll
         for (int i = 0; i < ST / 32; ++i)
         {
             mx = fmaxf(mx, __uint_as_float(sh.warp32[i]));
@@ -264,21 +312,30 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     {
         // nothing to pick, or the largest logit: its lowest id
         int id = a.V;
-        if (mx != NONE)
-            for (int j = tid; j < n; j += ST)
-                if (lg[j] == mx) { id = g0 + j; break; }
+        if (mx != NONE && mine_max == mx)
+            for (int j = tid * G; j < n && id == a.V; j += ST * G)
+                for (int q = G - 1; q >= 0; --q)
+                    if (lg[j + q] == mx) id = g0 + j + q;
         if (tid == 0) sh.id = a.V;
         __syncthreads();
         id = __reduce_min_sync(0xffffffffu, id);
         if (lane == 0) atomicMin(&sh.id, id);
         __syncthreads();
-        const int sl = exchange((u64) sh.id, 0);
+        const int sl = exchange((u64) sh.id);
         if (rank == 0 && tid == 0)
         {
             for (int r = 0; r < NC; ++r) id = min(id, (int) sh.mail[sl][0][r]);
             put(mx == NONE ? -1 : id);
         }
         return;
+    }
+    if (mx == INF)
+    {
+        // equal shares of the infinite logits: as if they were 0 and the others masked
+        for (int j = tid; j < n; j += ST) lg[j] = lg[j] == INF ? 0.0f : NONE;
+        mine_max = mine_max == INF ? 0.0f : NONE;
+        mx = mn = 0.0f;
+        __syncthreads();
     }
     Weight weight;
     weight.init(mx, T0);
@@ -288,9 +345,6 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     const u64 least = mp > 0.0 ? (u64) ceil(mp * 17592186044416.0) : 0ull;
     const double u = fmin(fmax((double) a.u[b], 0.0), 1.0);
     const bool by_k = k > 0 && k < a.V, by_p = top_p < 1.0f;
-    // bins of m - l (monotone in l); what lies beyond the span is in the last one
-    const float span = fminf(SPAN * T0, mx - mn), bscale = span > 0.0f ? 1023.9f / span : 0.0f;
-    auto bin_of = [&](float l) { return l == mx ? 0 : (int) fminf((mx - l) * bscale, 1023.0f); };
     auto need_of = [&](u64 S) {                            // the mass before which a logit stays: at least the first does
         const u64 v = top_p > 0.0f ? (u64) ceil((double) top_p * (double) S) : 1ull;
         return v < 1 ? 1ull : v;
@@ -299,72 +353,44 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         const u64 t = (u64) (u * (double) S);
         return t >= S ? S - 1 : t;
     };
-
-    // kept: key > thr, or key == thr and id <= cut
-    uint32_t thr = 0;
-    int cut = a.V;
-    auto kept = [&](uint32_t ky, int i) { return ky > thr || (ky == thr && i <= cut); };
-
-    // A histogram over the cluster of the kept logits for which bin(l, key) >= 0, and the bin at which the running sum of
-    // counts (mass: of weights) reaches `need` (frac: need_of the whole sum). total: the whole sum
-    auto histogram = [&](bool mass, bool frac, u64& need, u64& total, auto bin) {
-        Hist& h = sh.hist[hslot];
-        for (int i = tid; i < (int) (sizeof(Hist) / 4); i += ST) reinterpret_cast<uint32_t*>(&h)[i] = 0;
+    // bins of m - l (monotone in l); what lies beyond the span is in the last one
+    auto bin_scale = [&](float span) { return span > 0.0f ? 1023.9f / span : 0.0f; };
+    auto bin_at = [&](float l, float scale) { return l == mx ? 0 : (int) fminf((mx - l) * scale, 1023.0f); };
+    // f(logit, place in the slice) of this thread's share, the groups that it loaded
+    auto each = [&](auto f) {
+        for (int j = tid * G; j < n; j += ST * G)
+#pragma unroll
+            for (int q = 0; q < G / 4; ++q)
+            {
+                const int at = j + 4 * q;
+                const float4 v = *reinterpret_cast<const float4*>(lg + at);
+                f(v.x, at); f(v.y, at + 1); f(v.z, at + 2); f(v.w, at + 3);
+            }
+    };
+    // at most the smallest logit whose bin is `bin` or less: what is below it lies in a later bin
+    auto bin_floor = [&](int bin, float scale) {
+        return scale > 0.0f && bin < SBINS - 1 ? mx - (float) (bin + 1) / scale * (1.0f + 0x1p-18f) - fabsf(mx) * 0x1p-20f : NONE;
+    };
+    auto block_sum = [&](u64 v) {
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         __syncthreads();
-        for (int j = tid; j < n; j += ST)
-        {
-            const float l = lg[j];
-            if (l == NONE) continue;
-            const uint32_t ky = key_of<T>(l);
-            const int q = kept(ky, g0 + j) ? bin(l, ky) : -1;
-            if (q < 0) continue;
-            atomicAdd(&h.cnt[q], 1u);
-            if (mass)
-            {
-                const u64 w = weight(l);
-                const uint32_t wl = (uint32_t) w, wh = (uint32_t) (w >> 32);
-                if (wl)
-                {
-                    const uint32_t old = atomicAdd(&h.lo[q], wl);
-                    if (wh + (old + wl < old)) atomicAdd(&h.hi[q], wh + (old + wl < old));
-                }
-                else if (wh)
-                    atomicAdd(&h.hi[q], wh);
-            }
-        }
-        sync();
-        // bins 2 tid and 2 tid + 1 of all CTAs
-        u64 v0 = 0, v1 = 0;
-        uint32_t c0 = 0, c1 = 0;
-        for (int r = 0; r < NC; ++r)
-        {
-            const u64 c = dsmem_ld(&h.cnt[2 * tid], r);
-            c0 += (uint32_t) c;
-            c1 += (uint32_t) (c >> 32);
-            if (mass)
-            {
-                const u64 l = dsmem_ld(&h.lo[2 * tid], r), hi = dsmem_ld(&h.hi[2 * tid], r);
-                v0 += (l & 0xffffffffu) + (hi << 32);
-                v1 += (l >> 32) + (hi >> 32 << 32);
-            }
-        }
-        hslot ^= 1;
-        uint32_t call;
-        const uint32_t cs = block_scan(c0 + c1, sh.warp32, call);
-        if (!mass) { v0 = c0; v1 = c1; }
-        u64 vs = cs;
-        total = call;
-        if (mass) vs = block_scan(v0 + v1, sh.warp, total);
-        if (frac) need = need_of(total);
-        const u64 before = vs - v0 - v1;
-        if (before < need && vs >= need)
+        if (lane == 0) sh.warp[warp] = v;
+        __syncthreads();
+        u64 all = 0;
+#pragma unroll
+        for (int i = 0; i < ST / 32; ++i) all += sh.warp[i];
+        return all;
+    };
+    // the bin (of this thread's two) in which the running sum of v0, v1 reaches need
+    auto crossing = [&](u64 v0, u64 v1, u64 upto, u64 need, uint32_t c0, uint32_t c1) {
+        const u64 before = upto - v0 - v1;
+        if (before < need && upto >= need)
         {
             const bool second = before + v0 < need;
             Found f;
             f.bin = 2 * tid + second;
             f.above = before + (second ? v0 : 0);
             f.in = second ? v1 : v0;
-            f.cnt_above = cs - c0 - c1 + (second ? c0 : 0);
             f.cnt_in = second ? c1 : c0;
             sh.found = f;
         }
@@ -372,9 +398,147 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         return sh.found;
     };
 
+    u64 S = 0;                                             // the weights' sum, where top-p needs it
+    if (by_k || by_p)
+    {
+        // the edge: the bin at which k of the threads' maxima are reached (without a top-k, TRY of them or all)
+        const float scale = bin_scale(mx - mn);
+        if (mine_max != NONE) atomicAdd(&sh.maxima[bin_at(mine_max, scale)], 1u);
+        if (tid == 0) { sh.n_list = 0; sh.found.bin = -1; }
+        sync();
+        uint32_t c0 = 0, c1 = 0, all32;
+        {
+            u64 c[SRANKS];
+            dsmem_ld_all(&sh.maxima[2 * tid], NC, c);
+#pragma unroll
+            for (int r = 0; r < SRANKS; ++r) { c0 += (uint32_t) c[r]; c1 += (uint32_t) (c[r] >> 32); }
+        }
+        const uint32_t cs = block_scan(c0 + c1, sh.warp32, all32);
+        const uint32_t want = by_k ? (uint32_t) k : min(all32, (uint32_t) TRY);
+        const int edge = crossing(c0, c1, cs, want, c0, c1).bin;   // -1: fewer maxima than k
+        // gathered: what lies up to the edge (and a rounding more); with top-p alone, all weights are summed as well
+        u64 sum = 0, listed = 0;
+        int got = 0;
+        const float floor_l = edge >= 0 ? bin_floor(edge, scale) : INF;
+        auto gather = [&](float l, int j) {
+            if (l >= floor_l && l != NONE)
+            {
+                // straight into CTA 0's list, so that the others are done once their shares are in
+                const uint32_t at = dsmem_add(&sh.n_list, 0, 1u);
+                if (at < SLIST) dsmem_st(&sh.list[at], 0, (u64) __float_as_uint(l) << 32 | (uint32_t) (g0 + j));
+                ++got;
+                if (!by_k) listed += weight(l);
+            }
+        };
+        if (!by_k) each([&](float l, int j) { sum += weight(l); gather(l, j); });
+        else if (mine_max >= floor_l) each(gather);
+        got = __reduce_add_sync(0xffffffffu, got);
+        __syncthreads();
+        if (lane == 0) sh.warp32[warp] = got;
+        if (!by_k) { listed = block_sum(listed); sum = block_sum(sum); } else __syncthreads();
+        got = 0;
+#pragma unroll
+        for (int i = 0; i < ST / 32; ++i) got += sh.warp32[i];
+        const int sl = exchange((u64) got, sum, listed);
+        int total = 0;
+        listed = 0;
+        for (int r = 0; r < NC; ++r)
+        {
+            total += (int) sh.mail[sl][0][r];
+            S += sh.mail[sl][1][r];
+            listed += sh.mail[sl][2][r];
+        }
+        if (edge >= 0 && total <= SLIST && (by_k || listed >= need_of(S)))
+        {
+            if (rank == 0)
+            {
+                // the list is in any order: the sort fixes it
+                const bool in = tid < total;
+                const u64 e = in ? sh.list[tid] : 0ull;
+                // by key, then by id: descending (key, ~id); with the key of fp32, from which the logit comes back
+                u64 s = in ? (u64) key_of<float>(__uint_as_float((uint32_t) (e >> 32))) << 32 | (uint32_t) ~(uint32_t) e : 0ull;
+                s = sort_n(s, total, sh.sorted);
+                const uint32_t ky = (uint32_t) (s >> 32), id = ~(uint32_t) s;
+                const float l = of_key<float>(ky);
+                u64 w = in && (!by_k || tid < k) ? weight(l) : 0ull, all;
+                u64 upto = block_scan(w, sh.warp, all);
+                if (by_p && tid > 0 && upto - w >= need_of(by_k ? all : S)) w = 0;
+                if (w < least) w = 0;
+                // the pick, in id order
+                uint32_t o = w ? ((0x3fffffu - id) << 9 | (uint32_t) tid) : 0u;
+                __syncthreads();
+                sh.sorted[tid] = w;
+                o = sort_n(o, total, sh.order);
+                __syncthreads();
+                const u64 wo = o ? sh.sorted[o & 511] : 0ull;
+                upto = block_scan(wo, sh.warp, all);
+                const u64 target = target_of(all);
+                if (wo && upto - wo <= target && upto > target) put((int) (0x3fffffu - (o >> 9)));
+            }
+            return;
+        }
+    }
+
+    // ---- the general way: many logits are kept ----
+    // kept: l > thr, or l == thr and id <= cut
+    float thr = NONE;
+    int cut = a.V;
+    auto kept = [&](float l, int j) { return l > thr || (l == thr && g0 + j <= cut); };
+
+    // A histogram over the cluster of the kept logits for which bin(l) >= 0, and the bin at which the running sum of counts (mass: of
+    // weights, with the counts too where wanted) reaches `need`
+    auto histogram = [&](bool mass, bool counts, u64 need, auto bin) {
+        Hist& h = sh.hist;
+        sync();                                            // nobody reads an earlier one
+        for (int i = tid; i < (int) (sizeof(Hist) / 16); i += ST) reinterpret_cast<uint4*>(&h)[i] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) sh.found.bin = -1;
+        __syncthreads();
+        each([&](float l, int j) {
+            const int q = l != NONE && kept(l, j) ? bin(l) : -1;
+            if (q < 0) return;
+            if (!mass) { atomicAdd(&h.lo[lane & 3][q], 1u); return; }
+            if (counts) atomicAdd(&h.cnt[q], 1u);
+            const u64 w = weight(l);
+            const uint32_t wl = (uint32_t) w;
+            uint32_t up = (uint32_t) (w >> 32);
+            if (wl) up += atomicAdd(&h.lo[lane & 3][q], wl) > ~wl;   // the carry of the low word
+            if (up) atomicAdd(&h.hi[q], up);
+        });
+        __syncthreads();
+        // the copies into one
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+            const int q = 2 * tid + i;
+            const u64 t = (u64) h.lo[0][q] + h.lo[1][q] + h.lo[2][q] + h.lo[3][q];
+            h.lo[0][q] = (uint32_t) t;
+            h.hi[q] += (uint32_t) (t >> 32);
+        }
+        sync();
+        // bins 2 tid and 2 tid + 1 of all CTAs
+        u64 v0 = 0, v1 = 0, c[SRANKS], hi[SRANKS];
+        uint32_t c0 = 0, c1 = 0;
+        dsmem_ld_all(&h.lo[0][2 * tid], NC, c);
+        dsmem_ld_all(&h.hi[2 * tid], NC, hi);
+#pragma unroll
+        for (int r = 0; r < SRANKS; ++r)
+        {
+            v0 += (c[r] & 0xffffffffu) + (hi[r] << 32);
+            v1 += (c[r] >> 32) + (hi[r] >> 32 << 32);
+        }
+        if (counts)
+        {
+            dsmem_ld_all(&h.cnt[2 * tid], NC, c);
+#pragma unroll
+            for (int r = 0; r < SRANKS; ++r) { c0 += (uint32_t) c[r]; c1 += (uint32_t) (c[r] >> 32); }
+        }
+        u64 all;
+        const u64 upto = block_scan(v0 + v1, sh.warp, all);
+        return crossing(v0, v1, upto, need, mass ? c0 : (uint32_t) v0, mass ? c1 : (uint32_t) v1);
+    };
     // id order over the cluster: this CTA's share of a sum, the sums before it and of all
     auto spread = [&](u64 mine, u64& before, u64& all) {
-        const int sl = exchange(mine, 0);
+        const int sl = exchange(mine);
         before = all = 0;
         for (int r = 0; r < NC; ++r)
         {
@@ -383,60 +547,91 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
             all += v;
         }
     };
-    // this warp's run of the slice, in rows of 32
-    const int run = (n + ST - 1) / ST * 32, j0 = min(n, warp * run), j1 = min(n, j0 + run);
+    // this warp's run of the slice, in rows of 128: four a lane
+    const int run = (n + ST * 4 - 1) / (ST * 4) * 128, j0 = min(n, warp * run), j1 = min(n, j0 + run);
     // sum of f over the slice; `mine` gets this warp's part
     auto slice_sum = [&](auto f, u64& mine) {
         mine = 0;
-        for (int j = j0 + lane; j < j1; j += 32) mine += f(lg[j], g0 + j);
+#pragma unroll 2
+        for (int j = j0 + lane * 4; j < j1; j += 128)
+        {
+            const float4 v = *reinterpret_cast<const float4*>(lg + j);
+            mine += f(v.x, j) + f(v.y, j + 1) + f(v.z, j + 2) + f(v.w, j + 3);
+        }
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        u64 all;
-        const u64 s = block_scan(lane == 0 ? mine : 0ull, sh.warp, all);
-        (void) s;
-        return all;
+        return block_sum(lane == 0 ? mine : 0ull);
     };
-    // lowest id whose running sum exceeds target (the sums before this CTA given); only the warp that holds it calls put_id
+    // lowest id whose running sum exceeds target (the sum before this CTA given), after slice_sum: put_id is called by the lane that
+    // holds it, if it is in this CTA
     auto find = [&](auto f, u64 mine, u64 before, u64 target, auto put_id) {
         for (int i = 0; i < warp; ++i) before += sh.warp[i];
         if (before <= target && before + mine > target)
-            for (int q = j0; q < j1; q += 32)
+            for (int q = j0; q < j1; q += 128)
             {
-                const u64 c = warp_scan(q + lane < j1 ? f(lg[q + lane], g0 + q + lane) : 0ull, lane);
+                const int j = q + lane * 4;
+                u64 w[4] = {};
+                if (j < j1)
+                {
+                    const float4 v = *reinterpret_cast<const float4*>(lg + j);
+                    w[0] = f(v.x, j); w[1] = f(v.y, j + 1); w[2] = f(v.z, j + 2); w[3] = f(v.w, j + 3);
+                }
+                const u64 own = w[0] + w[1] + w[2] + w[3], c = warp_scan(own, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, before + c > target);
                 if (hit)
                 {
-                    if (lane == 0) put_id(g0 + q + __ffs(hit) - 1);
+                    if (lane == __ffs(hit) - 1)
+                    {
+                        u64 at = before + c - own;
+                        int i = 0;
+                        while (at + w[i] <= target) at += w[i++];
+                        put_id(g0 + j + i);
+                    }
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, c, 31);
             }
     };
 
-    // from the first histogram's bin to the exact threshold, in thr and cut
-    auto narrow = [&](bool mass, u64 need, Found f) {
+    // from a bin of m - l (of that scale) to the exact threshold, in thr and cut
+    auto narrow = [&](bool mass, u64 need, Found f, float scale) {
         const int b0 = f.bin;
         u64 above = f.above;
-        uint32_t lo = 0xffffffffu, hi = 0;
-        for (int j = tid; j < n; j += ST)
-        {
-            const float l = lg[j];
-            if (l == NONE || bin_of(l) != b0) continue;
+        uint32_t lo = 0xffffffffu, hi = 0, cnt = 0;
+        const float floor_l = bin_floor(b0, scale);
+        each([&](float l, int j) {
+            if (!(l >= floor_l) || l == NONE || bin_at(l, scale) != b0 || !kept(l, j)) return;
             const uint32_t ky = key_of<T>(l);
-            if (kept(ky, g0 + j)) { lo = min(lo, ky); hi = max(hi, ky); }
-        }
+            lo = min(lo, ky);
+            hi = max(hi, ky);
+            ++cnt;
+        });
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
+        cnt = __reduce_add_sync(0xffffffffu, cnt);
         __syncthreads();
-        if (lane == 0) { sh.warp32[warp] = lo; sh.warp[warp] = hi; }
+        if (lane == 0) { sh.warp32[warp] = lo; sh.warp[warp] = (u64) cnt << 32 | hi; }
         __syncthreads();
-        for (int i = 0; i < ST / 32; ++i) { lo = min(lo, sh.warp32[i]); hi = max(hi, (uint32_t) sh.warp[i]); }
-        const int sl = exchange(lo, hi);
-        for (int r = 0; r < NC; ++r) { lo = min(lo, (uint32_t) sh.mail[sl][0][r]); hi = max(hi, (uint32_t) sh.mail[sl][1][r]); }
+        cnt = 0;
+        for (int i = 0; i < ST / 32; ++i)
+        {
+            lo = min(lo, sh.warp32[i]);
+            hi = max(hi, (uint32_t) sh.warp[i]);
+            cnt += (uint32_t) (sh.warp[i] >> 32);
+        }
+        const int sl = exchange(lo, hi, cnt);
+        cnt = 0;
+        for (int r = 0; r < NC; ++r)
+        {
+            lo = min(lo, (uint32_t) sh.mail[sl][0][r]);
+            hi = max(hi, (uint32_t) sh.mail[sl][1][r]);
+            cnt += (uint32_t) sh.mail[sl][2][r];
+        }
+        f.cnt_in = cnt;
         while (lo < hi)
         {
             const int s = max(0, 32 - __clz(hi - lo) - 10);
-            u64 left = need - above, total;
-            f = histogram(mass, false, left, total, [&](float, uint32_t ky) { return ky >= lo && ky <= hi ? (int) ((hi - ky) >> s) : -1; });
+            const float lo_l = of_key<T>(lo), hi_l = of_key<T>(hi);
+            f = histogram(mass, true, need - above, [&](float l) { return l >= lo_l && l <= hi_l ? (int) ((hi - key_of<T>(l)) >> s) : -1; });
             above += f.above;
             hi -= (uint32_t) f.bin << s;
             lo = max(lo, hi - ((1u << s) - 1));
@@ -445,110 +640,70 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         const u64 w = mass ? f.in / f.cnt_in : 1ull;
         const u64 m = w ? (need - above + w - 1) / w : (u64) f.cnt_in;
         int c = a.V;
+        const float t = of_key<T>(hi);
         if (m < f.cnt_in)
         {
-            auto tie = [&](float l, int i) { const uint32_t ky = key_of<T>(l); return (u64) (l != NONE && ky == hi && kept(ky, i)); };
+            auto tie = [&](float l, int j) { return (u64) (l == t && kept(l, j)); };
             u64 mine, before, all;
             if (tid == 0) sh.id = 0;
             const u64 sum = slice_sum(tie, mine);
             spread(sum, before, all);
             find(tie, mine, before, m - 1, [&](int id) { sh.id = id + 1; });
             __syncthreads();
-            const int sl2 = exchange((u64) sh.id, 0);
+            const int sl2 = exchange((u64) sh.id);
             for (int r = 0; r < NC; ++r)
                 if (sh.mail[sl2][0][r]) c = (int) sh.mail[sl2][0][r] - 1;
         }
-        thr = hi;
+        else if (t == thr)
+            c = cut;
+        thr = t;
         cut = c;
     };
 
-    if (by_k || by_p)
+    if (by_k)
     {
-        u64 need = by_k ? (u64) k : 0, S;
-        auto first = [&](float l, uint32_t) { return bin_of(l); };
-        // fewer logits than k that may be picked at all: top-k keeps them
-        Found f;
-        bool done_k = !by_k;
-        if (tid == 0) sh.found.bin = -1;
-        if (by_k)
+        // bins over the whole row, from a pass for its smallest logit
+        float least_l = mx;
+        each([&](float l, int) { if (l != NONE) least_l = fminf(least_l, l); });
+        // order-preserving, so that the block's minimum is an integer one
+        uint32_t kl = key_of<float>(least_l);
+        kl = __reduce_min_sync(0xffffffffu, kl);
+        __syncthreads();
+        if (lane == 0) sh.warp32[warp] = kl;
+        __syncthreads();
+        for (int i = 0; i < ST / 32; ++i) kl = min(kl, sh.warp32[i]);
+        const int sl = exchange(kl);
+        for (int r = 0; r < NC; ++r) kl = min(kl, (uint32_t) sh.mail[sl][0][r]);
+        const float scale = bin_scale(mx - of_key<float>(kl));
+        const Found f = histogram(false, false, (u64) k, [&](float l) { return bin_at(l, scale); });
+        if (f.bin >= 0) narrow(false, (u64) k, f, scale);  // else: fewer than k logits may be picked at all
+        if (by_p)
         {
-            f = histogram(false, false, need, S, first);
-            if (f.bin < 0) done_k = true;
+            u64 mine, before;
+            const u64 sum = slice_sum([&](float l, int j) { return kept(l, j) ? weight(l) : 0ull; }, mine);
+            spread(sum, before, S);
         }
-        if (done_k && by_p) f = histogram(true, true, need, S, first);
-        if (!(done_k && !by_p) && f.cnt_above + f.cnt_in <= SLIST)
-        {
-            // few logits: gathered, sorted and finished in CTA 0
-            const int total = (int) (f.cnt_above + f.cnt_in);
-            if (tid == 0) sh.n_list = 0;
-            __syncthreads();
-            for (int j = tid; j < n; j += ST)
-            {
-                const float l = lg[j];
-                if (l == NONE || bin_of(l) > f.bin) continue;
-                sh.list[atomicAdd(&sh.n_list, 1)] = (u64) __float_as_uint(l) << 32 | (uint32_t) (g0 + j);
-            }
-            __syncthreads();
-            const int sl = exchange((u64) sh.n_list, 0);
-            if (rank == 0)
-            {
-                // element tid of the CTAs' lists, in any order: the sort fixes it
-                u64 e = 0;
-                int at = tid;
-                for (int r = 0; r < NC; ++r)
-                {
-                    const int c = (int) sh.mail[sl][0][r];
-                    if (at >= 0 && at < c) { e = dsmem_ld(&sh.list[at], r); at = -1; }
-                    else if (at >= 0) at -= c;
-                }
-                int N = 32;
-                while (N < total) N <<= 1;
-                const bool in = tid < total;
-                // by key, then by id: descending (key, ~id); with the key of fp32, from which the logit comes back
-                u64 s = in ? (u64) key_of<float>(__uint_as_float((uint32_t) (e >> 32))) << 32 | (uint32_t) ~(uint32_t) e : 0ull;
-                s = block_sort(s, N, sh.sorted);
-                const uint32_t ky = (uint32_t) (s >> 32), id = ~(uint32_t) s;
-                const float l = __uint_as_float(ky & 0x80000000u ? ky & 0x7fffffffu : ~ky);
-                u64 w = in && (!by_k || done_k || tid < k) ? weight(l) : 0ull, all;
-                u64 upto = block_scan(w, sh.warp, all);
-                if (by_p && tid > 0 && upto - w >= need_of(done_k ? S : all)) w = 0;
-                if (w < least) w = 0;
-                // the pick, in id order
-                uint32_t o = w ? ((0x3fffffu - id) << 9 | (uint32_t) tid) : 0u;
-                sh.order[tid] = 0;
-                __syncthreads();
-                sh.sorted[tid] = w;
-                o = block_sort(o, N, sh.order);
-                __syncthreads();
-                const u64 wo = o ? sh.sorted[o & 511] : 0ull;
-                upto = block_scan(wo, sh.warp, all);
-                const u64 target = target_of(all);
-                if (wo && upto - wo <= target && upto > target) put((int) (0x3fffffu - (o >> 9)));
-            }
-            sync();                                        // the lists are read
-            return;
-        }
-        if (!done_k)
-        {
-            narrow(false, need, f);
-            if (by_p)
-            {
-                f = histogram(true, true, need, S, first);
-                narrow(true, need, f);
-            }
-        }
-        else if (by_p)
-            narrow(true, need, f);
     }
-    auto final_weight = [&](float l, int i) {
-        if (l == NONE || !kept(key_of<T>(l), i)) return 0ull;
-        const u64 w = weight(l);
-        return w >= least ? w : 0ull;
-    };
+    if (by_p)
+    {
+        const u64 need = need_of(S);
+        const float scale = bin_scale(fminf(SPAN * T0, mx - fmaxf(thr, -3.0e38f)));
+        const Found f = histogram(true, false, need, [&](float l) { return bin_at(l, scale); });
+        narrow(true, need, f, scale);
+    }
     u64 mine, before, all;
-    const u64 sum = slice_sum(final_weight, mine);
-    spread(sum, before, all);
-    find(final_weight, mine, before, target_of(all), put);
+    auto pick = [&](auto final_weight) {
+        const u64 sum = slice_sum(final_weight, mine);
+        spread(sum, before, all);
+        find(final_weight, mine, before, target_of(all), put);
+    };
+    if (thr == NONE && !least) pick([&](float l, int) { return weight(l); });
+    else
+        pick([&](float l, int j) {
+            if (!kept(l, j)) return 0ull;
+            const u64 w = weight(l);
+            return w >= least ? w : 0ull;
+        });
 }
 
 template <typename T>
