@@ -9,7 +9,16 @@ static __device__ int g_dense_err;
 int dense_device()
 {
     int d = -1;
-    return cudaGetDevice(&d) == cudaSuccess ? d : -1;
+    if (cudaGetDevice(&d) != cudaSuccess) return -1;
+    // the tensor-map encoder is a driver call and needs the device's context current in this thread, which a thread's first
+    // runtime calls (an autograd worker's, say) need not have made it
+    static thread_local int bound = -1;
+    if (bound != d)
+    {
+        if (cudaSetDevice(d) != cudaSuccess) return -1;
+        bound = d;
+    }
+    return d;
 }
 
 cudaError_t dense_err_ptr(int** p)

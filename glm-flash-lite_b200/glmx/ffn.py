@@ -8,40 +8,42 @@ to capture into a graph); `gated_ffn` is the same as a differentiable function.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
 
 from . import _lib
 from ._lib import check
-from .layer import _dt, _stream_ptr
+from .layer import _dt
+
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream's handle, without a Stream object around it
 
 
-def _on(device: torch.device, stream):
-    """The context in which a call allocates and launches: tensors' device current, and `stream` (if given) current too,
-    so that its temporaries belong to the stream that uses them."""
+def _on(index: int, stream):
+    """The context in which a call allocates and launches: the tensors' device current, and `stream` (if given) current
+    too, so that its temporaries belong to the stream that uses them. None where nothing has to be switched."""
     if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"stream on {stream.device}, tensors on {device}")
+        if stream.device.index != index:
+            raise ValueError(f"stream on {stream.device}, tensors on cuda:{index}")
         return torch.cuda.stream(stream)
-    if device.index != torch.cuda.current_device():
-        return torch.cuda.device(device)
-    return contextlib.nullcontext()
+    if index != _current_device():
+        return torch.cuda.device(index)
+    return None
 
 
 def _rows(t: torch.Tensor, align: int) -> torch.Tensor:
     """t [R, n] as rows of packed elements whose distance is a multiple of `align` elements and whose start is 16-byte
     aligned; copied where it is not."""
-    if t.stride(1) != 1 or t.stride(0) % align or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
-        if t.shape[0] == 1 and t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.shape[1] % align == 0:
-            return t.as_strided(t.shape, (t.shape[1], 1))
-        n = t.shape[1]
-        pitch = (n + align - 1) // align * align
-        c = torch.empty((t.shape[0], pitch), dtype=t.dtype, device=t.device)[:, :n]
-        c.copy_(t)
-        return c
-    return t
+    pitch, inner = t.stride()
+    if inner == 1 and pitch % align == 0 and pitch >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    R, n = t.shape
+    if R == 1 and inner == 1 and n % align == 0 and t.data_ptr() % 16 == 0:
+        return t.as_strided((1, n), (n, 1))
+    c = torch.empty((R, (n + align - 1) // align * align), dtype=t.dtype, device=t.device)[:, :n]
+    c.copy_(t)
+    return c
 
 
 class GatedFFN:
@@ -65,7 +67,8 @@ class GatedFFN:
             raise ValueError("weights must be on a CUDA device (there is no CPU path)")
         if not act_limit >= 0.0:
             raise ValueError("act_limit must be 0 (none) or positive")
-        with _on(self.device, None):
+        self._index = w_gate.get_device()
+        with torch.cuda.device(self._index):
             pack = lambda w: w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
             self.w_gate, self.w_up, self.w_down = (pack(w.detach()) for w in (w_gate, w_up, w_down))
         self.act_limit = float(act_limit)
@@ -78,74 +81,88 @@ class GatedFFN:
             raise ValueError(f"{what} must be [..., {self.H}]")
         if x.dtype != self.dtype:
             raise TypeError(f"{what} must be {self.dtype}, not {x.dtype}")
-        if x.device != self.device:
+        if x.get_device() != self._index:
             raise ValueError(f"{what} on {x.device}, weights on {self.device}")
-        return x if x.dim() == 2 else x.reshape(-1, self.H)
+        return _rows(x if x.dim() == 2 else x.reshape(-1, self.H), 8)
 
-    def _forward(self, x, y, accumulate, h, p, q):
-        x = _rows(x, 8)
-        check(self.lib.glmx_ffn_forward(self._ref, x.data_ptr(), x.stride(0), x.shape[0], y.data_ptr(), y.stride(0), _dt(y),
-                                        int(accumulate), h.data_ptr(), p, q, _stream_ptr(None)))
+    def _new(self, shape, dtype=None):
+        return torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
+
+    def _run(self, x, y, accumulate, h, p, q):
+        rc = self.lib.glmx_ffn_forward(self._ref, x.data_ptr(), x.stride(0), x.shape[0], y.data_ptr(), self.H, _dt(y), accumulate,
+                                       h.data_ptr(), p, q, _raw_stream(self._index))
+        if rc:
+            check(rc)
 
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False,
                 stream=None) -> torch.Tensor:
         """y [..., H] for x [..., H] of the block's dtype. out_dtype: the block's dtype (default) or fp32; out: a
         contiguous tensor of x's shape to write instead, accumulate=True to add to it (a shared expert's output onto
         MoELayer.forward's)."""
-        with _on(self.device, stream):
-            x2 = self._in(x, "x")
-            if out is None:
-                if accumulate:
-                    raise ValueError("accumulate needs out")
-                dt = self.dtype if out_dtype is None else out_dtype
-                if dt not in (self.dtype, torch.float32):
-                    raise TypeError(f"out_dtype must be {self.dtype} or fp32")
-                out = torch.empty(x.shape, dtype=dt, device=self.device)
-            else:
-                if out.shape != x.shape or not out.is_contiguous() or out.device != self.device or out.data_ptr() % 16:
-                    raise ValueError("out must be contiguous, 16-byte aligned, of x's shape and device")
-                if out.dtype not in (self.dtype, torch.float32) or (out_dtype is not None and out_dtype != out.dtype):
-                    raise TypeError(f"out must be {self.dtype} or fp32")
-            if x2.shape[0]:
-                h = torch.empty((x2.shape[0], self.I), dtype=self.dtype, device=self.device)
-                self._forward(x2, out.view(-1, self.H), accumulate, h, None, None)
-            return out
+        ctx = _on(self._index, stream)
+        if ctx is not None:
+            with ctx:
+                return self.forward(x, out, out_dtype, accumulate)
+        x2 = self._in(x, "x")
+        if out is None:
+            if accumulate:
+                raise ValueError("accumulate needs out")
+            if out_dtype is not None and out_dtype not in (self.dtype, torch.float32):
+                raise TypeError(f"out_dtype must be {self.dtype} or fp32")
+            out = self._new(x.shape, out_dtype)
+        else:
+            if out.shape != x.shape or not out.is_contiguous() or out.device != self.device or out.data_ptr() % 16:
+                raise ValueError("out must be contiguous, 16-byte aligned, of x's shape and device")
+            if out.dtype not in (self.dtype, torch.float32) or (out_dtype is not None and out_dtype != out.dtype):
+                raise TypeError(f"out must be {self.dtype} or fp32")
+        n = x2.shape[0]
+        if n:
+            self._run(x2, out, 1 if accumulate else 0, self._new((n, self.I)), 0, 0)
+        return out
 
     __call__ = forward
 
     # ---- training -----------------------------------------------------------------------------------------------
     def forward_train(self, x: torch.Tensor, stream=None):
-        """(y, saved): y as forward's, and what backward needs: the packed input rows, the hidden rows and two fp32 factors per hidden
-        value (10 bytes for each, beside x)."""
-        with _on(self.device, stream):
-            x2 = _rows(self._in(x, "x"), 8)
-            n = x2.shape[0]
-            y = torch.empty(x.shape, dtype=self.dtype, device=self.device)
-            h = torch.empty((n, self.I), dtype=self.dtype, device=self.device)
-            pq = torch.empty((2, n, self.I), dtype=torch.float32, device=self.device)
-            if n:
-                self._forward(x2, y.view(-1, self.H), False, h, pq[0].data_ptr(), pq[1].data_ptr())
-            return y, (x2, h, pq)
+        """(y, saved): y as forward's, and what backward needs: the packed input rows, the hidden rows and two fp32 factors
+        per hidden value (10 bytes for each, beside x)."""
+        ctx = _on(self._index, stream)
+        if ctx is not None:
+            with ctx:
+                return self.forward_train(x)
+        x2 = self._in(x, "x")
+        n = x2.shape[0]
+        y, h, pq = self._new(x.shape), self._new((n, self.I)), self._new((2, n, self.I), torch.float32)
+        if n:
+            p = pq.data_ptr()
+            self._run(x2, y, 0, h, p, p + 4 * n * self.I)
+        return y, (x2, h, pq)
 
     def backward(self, dy: torch.Tensor, saved, need=(True, True, True, True), stream=None):
         """(dx, dw_gate, dw_up, dw_down) for dy [..., H] from forward_train's saved; None where need says so."""
-        with _on(self.device, stream):
-            dy2 = _rows(self._in(dy, "dy"), 8)
-            x, h, pq = saved
-            n = x.shape[0]
-            if dy2.shape[0] != n:
-                raise ValueError("dy must have the forward call's rows")
-            empty = lambda shape, want: torch.empty(shape, dtype=self.dtype, device=self.device) if want else None
-            dx = empty(dy.shape, need[0])
-            dwg, dwu, dwd = empty((self.I, self.H), need[1]), empty((self.I, self.H), need[2]), empty((self.H, self.I), need[3])
-            inner = any(need[:3]) and n
-            dgu = empty((2, n, self.I), inner)
-            ptr = lambda t: 0 if t is None else t.data_ptr()
-            check(self.lib.glmx_ffn_backward(self._ref, dy2.data_ptr(), dy2.stride(0) if n else self.H, x.data_ptr(),
-                                             x.stride(0) if n else self.H, n, h.data_ptr(), pq[0].data_ptr(), pq[1].data_ptr(),
-                                             dgu[0].data_ptr() if inner else 0, dgu[1].data_ptr() if inner else 0, ptr(dx),
-                                             ptr(dwg), ptr(dwu), ptr(dwd), _stream_ptr(None)))
-            return dx, dwg, dwu, dwd
+        ctx = _on(self._index, stream)
+        if ctx is not None:
+            with ctx:
+                return self.backward(dy, saved, need)
+        dy2 = self._in(dy, "dy")
+        x, h, pq = saved
+        n = x.shape[0]
+        if dy2.shape[0] != n:
+            raise ValueError("dy must have the forward call's rows")
+        H, I, new = self.H, self.I, self._new
+        dx = new(dy.shape) if need[0] else None
+        dwg = new((I, H)) if need[1] else None
+        dwu = new((I, H)) if need[2] else None
+        dwd = new((H, I)) if need[3] else None
+        inner = new((2, n, I)) if n and (need[0] or need[1] or need[2]) else None
+        ptr = lambda t: 0 if t is None else t.data_ptr()
+        p, g = pq.data_ptr(), ptr(inner)
+        rc = self.lib.glmx_ffn_backward(self._ref, dy2.data_ptr(), dy2.stride(0) if n else H, x.data_ptr(), x.stride(0) if n else H, n,
+                                        h.data_ptr(), p, p + 4 * n * I, g, g and g + 2 * n * I, ptr(dx), ptr(dwg), ptr(dwu),
+                                        ptr(dwd), _raw_stream(self._index))
+        if rc:
+            check(rc)
+        return dx, dwg, dwu, dwd
 
 
 class _GatedFFNFunction(torch.autograd.Function):
@@ -160,15 +177,14 @@ class _GatedFFNFunction(torch.autograd.Function):
                                "GatedFFN.backward")
         y, (x2, h, pq) = ffn.forward_train(x)
         ctx.save_for_backward(x2, h, pq, w_gate, w_up, w_down)
-        ctx.act_limit = act_limit
+        ctx.ffn = ffn
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x2, h, pq, w_gate, w_up, w_down = ctx.saved_tensors
-        ffn = GatedFFN(w_gate, w_up, w_down, ctx.act_limit)
-        return (*ffn.backward(dy, (x2, h, pq), ctx.needs_input_grad[:4]), None)
+        x2, h, pq = ctx.saved_tensors[:3]            # (and an error here where a weight was changed in between)
+        return (*ctx.ffn.backward(dy, (x2, h, pq), ctx.needs_input_grad), None)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,

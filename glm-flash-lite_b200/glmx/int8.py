@@ -11,8 +11,8 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .ffn import _on, _rows
-from .layer import _dt, _stream_ptr
+from .ffn import _on, _raw_stream, _rows
+from .layer import _dt
 
 _FLOAT = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -25,22 +25,30 @@ def quantize_rows(x: torch.Tensor, stream=None):
         raise ValueError("x must be [..., K] with K >= 1")
     if x.dtype not in _FLOAT:
         raise TypeError(f"x must be fp16, bf16 or fp32, not {x.dtype}")
-    if x.device.type != "cuda":
+    index = x.get_device()
+    if index < 0:
         raise ValueError("x must be on a CUDA device (there is no CPU path)")
-    with _on(x.device, stream):
-        K = x.shape[-1]
-        x2 = x if x.dim() == 2 else x.reshape(-1, K)
-        if x2.stride(1) != 1 or x2.stride(0) < K:
-            x2 = x2.contiguous()
-        R = x2.shape[0]
-        pitch = (K + 15) // 16 * 16
-        q = torch.empty((R, pitch), dtype=torch.int8, device=x.device)
-        s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        check(_lib.load().glmx_quantize_rows(x2.data_ptr(), _dt(x2), max(x2.stride(0), K), R, K, q.data_ptr(), pitch,
-                                             s.data_ptr(), _stream_ptr(None)))
-        if x.dim() != 2:
-            q = q.view(*x.shape[:-1], pitch)
-        return (q if pitch == K else q[..., :K]), s
+    ctx = _on(index, stream)
+    if ctx is not None:
+        with ctx:
+            return quantize_rows(x)
+    shape = x.shape
+    K = shape[-1]
+    x2 = x if len(shape) == 2 else x.reshape(-1, K)
+    pitch, inner = x2.stride()
+    if inner != 1 or pitch < K:
+        x2 = x2.contiguous()
+        pitch = K
+    R = x2.shape[0]
+    qp = (K + 15) // 16 * 16
+    q = torch.empty((R, qp), dtype=torch.int8, device=x.device)
+    s = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    rc = _lib.load().glmx_quantize_rows(x2.data_ptr(), _dt(x2), pitch, R, K, q.data_ptr(), qp, s.data_ptr(), _raw_stream(index))
+    if rc:
+        check(rc)
+    if len(shape) != 2:
+        q = q.view(*shape[:-1], qp)
+    return (q if qp == K else q[..., :K]), s
 
 
 def _q_rows(t: torch.Tensor, what: str, K: int) -> torch.Tensor:
@@ -59,7 +67,7 @@ def _collapses(t: torch.Tensor) -> bool:
 
 
 def _vec(t: torch.Tensor, n: int, what: str, device) -> torch.Tensor:
-    if t.dtype != torch.float32 or t.numel() != n or t.device != device:
+    if t.dtype != torch.float32 or t.numel() != n or t.get_device() != device.index:
         raise ValueError(f"{what} must be fp32 with {n} elements on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -80,10 +88,13 @@ class Int8Linear:
             raise TypeError("out_dtype must be fp16, bf16 or fp32")
         self.N, self.K = int(wq.shape[0]), int(wq.shape[1])
         self.device, self.out_dtype = wq.device, out_dtype
-        with _on(self.device, None):
+        self._index = wq.get_device()
+        with torch.cuda.device(self._index):
             self.wq = _rows(wq, 16)
             self.w_scale = _vec(w_scale, self.N, "w_scale", self.device)
             self.bias = None if bias is None else _vec(bias, self.N, "bias", self.device)
+        self._w, self._ldw, self._ws = self.wq.data_ptr(), self.wq.stride(0), self.w_scale.data_ptr()
+        self._bias = 0 if bias is None else self.bias.data_ptr()
 
     @classmethod
     def from_weight(cls, w: torch.Tensor, bias: torch.Tensor | None = None, out_dtype=None):
@@ -95,30 +106,38 @@ class Int8Linear:
                stream=None) -> torch.Tensor:
         """y [..., N] from quantised rows xq int8 [..., K] and x_scale fp32 [...] (quantize_rows' results: one
         quantisation serves several linears)."""
-        if xq.device != self.device:
+        if xq.get_device() != self._index:
             raise ValueError(f"xq on {xq.device}, weights on {self.device}")
-        with _on(self.device, stream):
-            x2 = _q_rows(xq, "xq", self.K)
-            T = x2.shape[0]
-            xs = _vec(x_scale, T, "x_scale", self.device)
-            if out is None:
-                dt = out_dtype or self.out_dtype or torch.bfloat16
-                if dt not in _FLOAT:
-                    raise TypeError("out_dtype must be fp16, bf16 or fp32")
-                out = torch.empty((*xq.shape[:-1], self.N), dtype=dt, device=self.device)
-            elif tuple(out.shape) != (*xq.shape[:-1], self.N) or not out.is_contiguous() or out.device != self.device or \
-                    out.dtype not in _FLOAT:
-                raise ValueError("out must be contiguous fp16 / bf16 / fp32 [..., N] on the weights' device")
-            check(self.lib.glmx_linear_i8(x2.data_ptr(), x2.stride(0) if T else self.wq.stride(0), xs.data_ptr(), T, self.K,
-                                          self.N, self.wq.data_ptr(), self.wq.stride(0), self.w_scale.data_ptr(),
-                                          0 if self.bias is None else self.bias.data_ptr(), out.data_ptr(), self.N, _dt(out),
-                                          _stream_ptr(None)))
-            return out
+        ctx = _on(self._index, stream)
+        if ctx is not None:
+            with ctx:
+                return self.matmul(xq, x_scale, out, out_dtype)
+        x2 = _q_rows(xq, "xq", self.K)
+        T = x2.shape[0]
+        xs = _vec(x_scale, T, "x_scale", self.device)
+        if out is None:
+            dt = out_dtype or self.out_dtype or torch.bfloat16
+            if dt not in _FLOAT:
+                raise TypeError("out_dtype must be fp16, bf16 or fp32")
+            out = torch.empty((*xq.shape[:-1], self.N), dtype=dt, device=self.device)
+        elif tuple(out.shape) != (*xq.shape[:-1], self.N) or not out.is_contiguous() or out.device != self.device or \
+                out.dtype not in _FLOAT:
+            raise ValueError("out must be contiguous fp16 / bf16 / fp32 [..., N] on the weights' device")
+        rc = self.lib.glmx_linear_i8(x2.data_ptr(), x2.stride(0) if T else self._ldw, xs.data_ptr(), T, self.K, self.N, self._w, self._ldw,
+                                     self._ws, self._bias, out.data_ptr(), self.N, _dt(out), _raw_stream(self._index))
+        if rc:
+            check(rc)
+        return out
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         """y [..., N] from x [..., K]: quantises the rows, then multiplies."""
         if x.shape[-1] != self.K:
             raise ValueError(f"x must be [..., {self.K}]")
-        with _on(self.device, stream):
-            q, s = quantize_rows(x)
-            return self.matmul(q, s, out, self.out_dtype or x.dtype)
+        if x.get_device() != self._index:
+            raise ValueError(f"x on {x.device}, weights on {self.device}")
+        ctx = _on(self._index, stream)
+        if ctx is not None:
+            with ctx:
+                return self(x, out)
+        q, s = quantize_rows(x)
+        return self.matmul(q, s, out, self.out_dtype or x.dtype)

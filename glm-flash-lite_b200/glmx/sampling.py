@@ -6,21 +6,21 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .ffn import _on
-from .layer import _dt, _stream_ptr
+from .ffn import _on, _raw_stream
+from .layer import _dt
 
 
-def _param(v, default, dtype, B: int, device, what: str):
-    """(tensor or None, its device address, the value for all rows)"""
+def _param(v, dtype, B: int, index: int, what: str):
+    """v, a number or a tensor [B], as (tensor kept alive, its device address or 0, the value for all rows)"""
     if not isinstance(v, torch.Tensor):
-        return None, 0, default if v is None else v
+        return None, 0, v
     if v.dim() == 0:
         v = v.expand(B)
-    if tuple(v.shape) != (B,) or v.device != device:
-        raise ValueError(f"{what} must be a number or a tensor [{B}] on {device}")
+    if tuple(v.shape) != (B,) or v.get_device() != index:
+        raise ValueError(f"{what} must be a number or a tensor [{B}] on cuda:{index}")
     if v.dtype != dtype or not v.is_contiguous():
         v = v.to(dtype).contiguous()
-    return v, v.data_ptr(), default
+    return v, v.data_ptr(), 0
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out_dtype=torch.int64,
@@ -41,22 +41,30 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         raise ValueError(f"at most {_lib.SAMPLE_MAX_VOCAB} logits a row")
     if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f"logits must be fp16, bf16 or fp32, not {logits.dtype}")
-    dev = logits.device
-    if dev.type != "cuda":
+    index = logits.get_device()
+    if index < 0:
         raise ValueError("logits must be on a CUDA device (there is no CPU path)")
     if out_dtype not in (torch.int64, torch.int32):
         raise TypeError("out_dtype must be int64 or int32")
-    if u.dtype != torch.float32 or tuple(u.shape) != (B,) or u.device != dev:
-        raise ValueError(f"u must be fp32 [{B}] on {dev}")
-    with _on(dev, stream):
-        if logits.stride(1) != 1 or (B > 1 and logits.stride(0) < V):
-            logits = logits.contiguous()
-        u = u if u.is_contiguous() else u.contiguous()
-        t, tp, t0 = _param(temperature, 1.0, torch.float32, B, dev, "temperature")
-        k, kp, k0 = _param(top_k, 0, torch.int32, B, dev, "top_k")
-        p, pp, p0 = _param(top_p, 1.0, torch.float32, B, dev, "top_p")
-        m, mp, m0 = _param(min_p, 0.0, torch.float32, B, dev, "min_p")
-        ids = torch.empty(B, dtype=out_dtype, device=dev)
-        check(_lib.load().glmx_sample(logits.data_ptr(), _dt(logits), max(logits.stride(0), V), B, V, u.data_ptr(), tp, t0, kp,
-                                      k0, pp, p0, mp, m0, ids.data_ptr(), _dt(ids), _stream_ptr(None)))
-        return ids
+    if u.dtype != torch.float32 or tuple(u.shape) != (B,) or u.get_device() != index:
+        raise ValueError(f"u must be fp32 [{B}] on cuda:{index}")
+    ctx = _on(index, stream)
+    if ctx is not None:
+        with ctx:
+            return sample(logits, u, temperature, top_k, top_p, min_p, out_dtype)
+    ld, inner = logits.stride()
+    if inner != 1 or (B > 1 and ld < V):
+        logits = logits.contiguous()
+        ld = V
+    if not u.is_contiguous():
+        u = u.contiguous()
+    t, tp, t0 = _param(temperature, torch.float32, B, index, "temperature")
+    k, kp, k0 = _param(top_k, torch.int32, B, index, "top_k")
+    p, pp, p0 = _param(top_p, torch.float32, B, index, "top_p")
+    m, mp, m0 = _param(min_p, torch.float32, B, index, "min_p")
+    ids = torch.empty(B, dtype=out_dtype, device=logits.device)
+    rc = _lib.load().glmx_sample(logits.data_ptr(), _dt(logits), max(ld, V), B, V, u.data_ptr(), tp, t0, kp, k0, pp, p0, mp, m0,
+                                 ids.data_ptr(), _dt(ids), _raw_stream(index))
+    if rc:
+        check(rc)
+    return ids

@@ -605,6 +605,29 @@ def test_streams(dev):
         assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
+def test_first_call_of_a_thread(dev):
+    """A thread that has made no CUDA call of its own (an autograd worker) may make its first one here."""
+    import threading
+    from glmx import GatedFFN, Int8Linear, sample
+    x, wg, wu, wd, dy = block(dev, 3, 64, 64, BF, 91)
+    ffn, lin = GatedFFN(wg, wu, wd), Int8Linear.from_weight(wg)
+    u = torch.rand(3, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    _, saved = ffn.forward_train(x)
+    calls = [lambda: ffn(x), lambda: lin(x), lambda: sample(x, u), lambda: ffn.backward(dy, saved)[0]]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    got = [None] * len(calls)
+
+    def run(i):
+        got[i] = calls[i]()
+        torch.cuda.synchronize()
+    for i in range(len(calls)):
+        t = threading.Thread(target=run, args=(i,))
+        t.start()
+        t.join()
+    assert all(g is not None and torch.equal(g, w) for g, w in zip(got, want))
+
+
 def test_refusals_with_device_tensors(dev):
     from glmx import GatedFFN, Int8Linear, gated_ffn, quantize_rows, sample
     x, wg, wu, wd, dy = block(dev, 4, 64, 32, BF, 81)
