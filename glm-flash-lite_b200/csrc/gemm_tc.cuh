@@ -24,7 +24,7 @@ struct Epi
 {
     int M, N;
     int bf16;                   // 16-bit type: bf16 or fp16
-    int vec;                    // rows of every output can take 16-byte stores
+    int vec;                    // rows of every output can take 16-byte stores (always but for I8 with an odd width)
     void* y; long long ldy; int y_dtype, accumulate;     // STORE, I8
     void* o0; void* o1;         // GATED: o0 = h; DACT: o0 = dg, o1 = du, [M][N]
     float* p; float* q;
@@ -51,8 +51,7 @@ __device__ __forceinline__ void store16(void* base, size_t off, const float (&v)
         }
     }
     uint8_t* d = static_cast<uint8_t*>(base) + off * 2;
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
 }
 
 __device__ __forceinline__ float load16(const void* base, size_t off, int bf16)
@@ -67,14 +66,14 @@ __device__ __forceinline__ void store_f32(float* d, const float (&v)[W])
     for (int i = 0; i < W / 4; ++i) reinterpret_cast<float4*>(d)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
 
-// W (4 or 8) consecutive columns n .. n + W - 1 of token t; n is a multiple of W. v: the sums (GATED: of gate; u of up).
-// I8 sums are int32 bit patterns.
+// W (4, or 1 where rows cannot take wide stores) consecutive columns n .. n + W - 1 of token t; n is a multiple of W. acc: the sums (GATED: of
+// gate; acc2 of up). I8 sums are int32 bit patterns.
 template <int EPI, int W>
 __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t (&acc)[W], const uint32_t (&acc2)[W])
 {
     if (t >= e.M || n >= e.N) return;
     float v[W];
-    if constexpr (EPI == EPI_GATED)
+    if constexpr (EPI == EPI_GATED && W == 4)
     {
         // N is a multiple of 8: all W columns are inside
         const size_t o = (size_t) t * e.N + n;
@@ -97,7 +96,7 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
         if (e.p) { store_f32<W>(e.p + o, pp); store_f32<W>(e.q + o, qq); }
         return;
     }
-    if constexpr (EPI == EPI_DACT)
+    if constexpr (EPI == EPI_DACT && W == 4)
     {
         const size_t o = (size_t) t * e.N + n;
         float dg[W], du[W];
@@ -136,15 +135,16 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
     }
     const size_t o = (size_t) t * e.ldy + n;
     const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
-    if (e.vec && n + W <= e.N)
-    {
-        if (e.accumulate)
+    if constexpr (W == 4)
+        if (e.vec && n + W <= e.N)
+        {
+            if (e.accumulate)
 #pragma unroll
-            for (int i = 0; i < W; ++i) v[i] += f32 ? static_cast<const float*>(e.y)[o + i] : load16(e.y, o + i, bf);
-        if (f32) store_f32<W>(static_cast<float*>(e.y) + o, v);
-        else store16<W>(e.y, o, v, bf);
-        return;
-    }
+                for (int i = 0; i < W; ++i) v[i] += f32 ? static_cast<const float*>(e.y)[o + i] : load16(e.y, o + i, bf);
+            if (f32) store_f32<W>(static_cast<float*>(e.y) + o, v);
+            else store16<W>(e.y, o, v, bf);
+            return;
+        }
 #pragma unroll
     for (int i = 0; i < W; ++i)
     {
@@ -311,13 +311,14 @@ constexpr int PAIR_EPI = 8;                              // epilogue warps: two 
 constexpr int PAIR_THREADS = (2 + PAIR_EPI) * 32;
 constexpr int PAIR_STAGES_MAX = 8;
 constexpr int PAIR_SMEM = 227 * 1024;
+constexpr int PAIR_STG = PAIR_EPI * 4096;                // the epilogue warps' staging
 constexpr int pair_stage(int bn) { return PAIR_BM * 128 + bn / 2 * 128; }
 constexpr int pair_stages(int bn)
 {
-    const int n = (PAIR_SMEM - 1024 - 2048) / pair_stage(bn);   // 1 KB of static shared memory, 2 KB of alignment
+    const int n = (PAIR_SMEM - 1024 - 1024 - PAIR_STG) / pair_stage(bn);   // 1 KB of static shared memory, 1 KB of alignment
     return n > PAIR_STAGES_MAX ? PAIR_STAGES_MAX : n;
 }
-constexpr int pair_smem(int bn) { return 2048 + pair_stages(bn) * pair_stage(bn); }
+constexpr int pair_smem(int bn) { return 1024 + pair_stages(bn) * pair_stage(bn) + PAIR_STG; }
 
 // I8: signed bytes; A_MN / B_MN: operand stored [K][rows]; EPI
 template <bool I8, bool A_MN, bool B_MN, int EPI>
@@ -430,6 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     else
     {
         const int q = warp & 3, half = (warp - 2) >> 2;
+        uint4* stg = reinterpret_cast<uint4*>(smem + (size_t) NST * STAGE) + (warp - 2) * 256;   // 4 KB: 32 rows of 128 bytes
         int lt = 0;
         for (int t = first; t < ntiles && !s_abort; t += pairs, ++lt)
         {
@@ -439,25 +441,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             if (!mbar_wait_bounded(&tfull[acc], (uint32_t) ((lt >> 1) & 1))) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
             tc_after();
             const Epi& e = a.e[p];
-            const int row = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q + lane;
             const uint32_t tq = tmem + ((uint32_t) (32 * q) << 16) + (uint32_t) (acc * 256);
-            // this warp's half of the tile's columns, 16 at a time
+            // this warp's half of the tile's columns, 32 at a time (GATED: 16 of gate and of up): a lane holds a row, and through shared memory
+            // each 8 (4) lanes get 4 columns each of one row, so that global accesses run along rows
             const int cols = EPI == EPI_GATED ? BN / 4 : BN / 2, c0 = half * cols;
-            for (int c = c0; c < c0 + cols; c += 16)
+            constexpr int CC = EPI == EPI_GATED ? 16 : 32, LPR = CC / 4;
+            for (int c = c0; c < c0 + cols; c += CC)
             {
                 uint32_t v[16], u[16];
                 tc_ld16(tq + (uint32_t) c, v);
-                if constexpr (EPI == EPI_GATED) tc_ld16(tq + (uint32_t) (BN / 2 + c), u);
+                tc_ld16(tq + (uint32_t) (EPI == EPI_GATED ? BN / 2 + c : c + 16), u);
                 tc_wait_ld();
-                const int nn = n * (EPI == EPI_GATED ? BN / 2 : BN) + c;
+                // 16-byte piece i of row r sits at place i ^ (r & 7)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int i = 0; i < 4; ++i)
                 {
-                    uint32_t v8[8], u8[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { v8[i] = v[8 * j + i]; u8[i] = EPI == EPI_GATED ? u[8 * j + i] : 0; }
-                    emit<EPI, 8>(e, row, nn + 8 * j, v8, u8);
+                    stg[lane * 8 + (i ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    stg[lane * 8 + ((i + 4) ^ (lane & 7))] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
                 }
+                __syncwarp();
+                const int nn = n * (EPI == EPI_GATED ? BN / 2 : BN) + c, row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
+                if (EPI != EPI_I8 || e.vec)
+                {
+#pragma unroll
+                    for (int i = 0; i < LPR; ++i)
+                    {
+                        const int r = i * (32 / LPR) + lane / LPR, pc = lane % LPR;
+                        const uint4 x = stg[r * 8 + (pc ^ (r & 7))], y = EPI == EPI_GATED ? stg[r * 8 + ((pc + 4) ^ (r & 7))] : x;
+                        const uint32_t x4[4] = { x.x, x.y, x.z, x.w }, y4[4] = { y.x, y.y, y.z, y.w };
+                        emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4, y4);
+                    }
+                }
+                else
+                {
+                    // rows that no wide store fits: a lane a column
+                    for (int r = 0; r < 32; ++r)
+                    {
+                        const uint32_t x1[1] = { reinterpret_cast<const uint32_t*>(stg)[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4 + (lane & 3)] };
+                        emit<EPI, 1>(e, row0 + r, nn + lane, x1, x1);
+                    }
+                }
+                __syncwarp();
             }
             tc_before();
             __syncwarp();
@@ -477,6 +501,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 }
 
 // ---- cols_kernel -------------------------------------------------------------------------------------------------------
+
+template <int N> struct Int { static constexpr int value = N; };
 
 struct ColsMaps
 {
@@ -511,47 +537,49 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
     const int splits = gridDim.x, split = blockIdx.x;      // one cluster along x
     const int mtile = blockIdx.y % a.mtiles, ttile = blockIdx.y / a.mtiles;
     const int NT = a.NT, NST = a.stages, STAGE = 16384 + NT * 128;
+    const int ksteps = (a.K + a.bk - 1) / a.bk, nk_all = ksteps * a.nseg;
+    const int k0 = (int) ((long long) nk_all * split / splits), nk = (int) ((long long) nk_all * (split + 1) / splits) - k0;
+    const int rows = EPI == EPI_GATED ? 64 : 128;          // output columns (weight rows of one matrix) per tile
+    auto load_w = [&](int i) {
+        const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
+        uint8_t* sw = smem + (size_t) s * STAGE;
+        mbar_arrive_expect_tx(&full[s], (uint32_t) STAGE);
+        if constexpr (EPI == EPI_GATED)
+            for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[j], kc, mtile * 64, &full[s]);
+        else if constexpr (W_MN)
+            for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[seg], mtile * 128 + 64 * j, kc, &full[s]);
+        else
+            tma_load_2d(sw, &maps.w[seg], kc, mtile * 128, &full[s]);
+    };
+    auto load_x = [&](int i) {
+        const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
+        tma_load_2d(smem + (size_t) s * STAGE + 16384, &maps.x[seg], kc, ttile * NT, &full[s]);
+    };
+    const int ahead = nk < NST ? nk : NST;                 // stages that need no wait
     if (tid == 0)
     {
         for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(&tfull, 1);
         s_abort = 0;
         fence_barrier_init();
+        // the first loads do not wait for the rest of the CTA
+        if (!a.prefetch) grid_wait();
+        for (int i = 0; i < ahead; ++i) load_w(i);
+        if (a.prefetch) grid_wait();
+        for (int i = 0; i < ahead; ++i) load_x(i);
     }
     if (warp == 1) tc_alloc<1>(&tmem_slot, (uint32_t) a.tcols);
+    __syncwarp();
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_slot;
     grid_release();
 
-    const int ksteps = (a.K + a.bk - 1) / a.bk, nk_all = ksteps * a.nseg;
-    const int k0 = (int) ((long long) nk_all * split / splits), nk = (int) ((long long) nk_all * (split + 1) / splits) - k0;
-    const int rows = EPI == EPI_GATED ? 64 : 128;          // output columns (weight rows of one matrix) per tile
-
     if (warp == 0)
     {
         if (lane == 0)
         {
-            auto load_w = [&](int i) {
-                const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
-                uint8_t* sw = smem + (size_t) s * STAGE;
-                mbar_arrive_expect_tx(&full[s], (uint32_t) STAGE);
-                if constexpr (EPI == EPI_GATED)
-                    for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[j], kc, mtile * 64, &full[s]);
-                else if constexpr (W_MN)
-                    for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[seg], mtile * 128 + 64 * j, kc, &full[s]);
-                else
-                    tma_load_2d(sw, &maps.w[seg], kc, mtile * 128, &full[s]);
-            };
-            auto load_x = [&](int i) {
-                const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
-                tma_load_2d(smem + (size_t) s * STAGE + 16384, &maps.x[seg], kc, ttile * NT, &full[s]);
-            };
-            const int ahead = a.prefetch ? (nk < NST ? nk : NST) : 0;
-            for (int i = 0; i < ahead; ++i) load_w(i);
-            grid_wait();
-            for (int i = 0; i < ahead; ++i) load_x(i);
             for (int i = ahead; i < nk; ++i)
             {
                 const int s = i % NST;
@@ -609,28 +637,48 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
         tc_after();
         tc_dealloc<1>(tmem, (uint32_t) a.tcols);
     }
-    // groups of 4 weight rows of one token, spread over the cluster's CTAs; partials are added in rank order
-    const int per = rows / 4, units = ncols * per;
-    const int u0 = (int) ((long long) units * split / splits), u1 = (int) ((long long) units * (split + 1) / splits);
+    // Spread over the cluster's CTAs: units of 4 weight rows of one token (or, where the output's rows take no wide stores, of single ones).
+    // A unit's partials are fetched from all CTAs at once and added in rank order.
     const uint32_t base = smem_u32(part);
-    if (!s_abort)
+    auto join = [&](auto wide) {
+        constexpr int W = decltype(wide)::value;
+        const int per = rows / W, units = ncols * per;
+        const int u0 = (int) ((long long) units * split / splits), u1 = (int) ((long long) units * (split + 1) / splits);
         for (int u = u0 + tid; u < u1; u += COLS_THREADS)
         {
-            const int c = u / per, r = (u - c * per) * 4;
-            uint32_t v[4] = {}, w[4] = {};
-            auto add = [&](uint32_t (&d)[4], uint32_t off, int rk) {
-                uint32_t x[4];
-                asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(map_rank(base + off, (uint32_t) rk)) : "memory");
+            const int c = u / per, r = (u - c * per) * W;
+            uint32_t v[W], w[W];
+            auto sum = [&](uint32_t (&d)[W], uint32_t off) {
+                uint32_t x[8][W];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[i] = rk == 0 ? x[i] : I8 ? d[i] + x[i] : __float_as_uint(__fadd_rn(__uint_as_float(d[i]), __uint_as_float(x[i])));
+                for (int rk = 0; rk < 8; ++rk)
+                    if (rk < splits)
+                    {
+                        const uint32_t at = map_rank(base + off, (uint32_t) rk);
+                        if constexpr (W == 4) asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[rk][0]), "=r"(x[rk][1]), "=r"(x[rk][2]), "=r"(x[rk][3]) : "r"(at));
+                        else asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x[rk][0]) : "r"(at));
+                    }
+#pragma unroll
+                for (int i = 0; i < W; ++i) d[i] = x[0][i];
+#pragma unroll
+                for (int rk = 1; rk < 8; ++rk)
+                    if (rk < splits)
+#pragma unroll
+                        for (int i = 0; i < W; ++i) d[i] = I8 ? d[i] + x[rk][i] : __float_as_uint(__fadd_rn(__uint_as_float(d[i]), __uint_as_float(x[rk][i])));
             };
-            for (int rk = 0; rk < splits; ++rk)
-            {
-                add(v, (uint32_t) (c * 128 + r) * 4, rk);
-                if constexpr (EPI == EPI_GATED) add(w, (uint32_t) (c * 128 + 64 + r) * 4, rk);
-            }
-            emit<EPI, 4>(a.e, ttile * NT + c, mtile * rows + r, v, w);
+            sum(v, (uint32_t) (c * 128 + r) * 4);
+            if constexpr (EPI == EPI_GATED) sum(w, (uint32_t) (c * 128 + 64 + r) * 4);
+            else
+#pragma unroll
+                for (int i = 0; i < W; ++i) w[i] = v[i];
+            emit<EPI, W>(a.e, ttile * NT + c, mtile * rows + r, v, w);
         }
+    };
+    if (!s_abort)
+    {
+        if (EPI == EPI_I8 && !a.e.vec) join(Int<1>());
+        else join(Int<4>());
+    }
     __syncwarp();
     if (splits > 1) cluster_sync();                        // nobody leaves while its partial tile is read
 }
