@@ -64,13 +64,13 @@ cudaError_t dense_map(CUtensorMap* m, int dtype, const Mat& t, int box_inner, in
             fn = reinterpret_cast<EncodeTiledFn>(p);
         if (!fn) return cudaErrorNotSupported;
     }
-    const bool bytes = dtype != GLMX_F16 && dtype != GLMX_BF16;
+    const int size = dtype == GLMX_F32 ? 4 : dtype == GLMX_F16 || dtype == GLMX_BF16 ? 2 : 1;
     const cuuint64_t dims[2] = { (cuuint64_t) t.inner, (cuuint64_t) t.rows };
-    const cuuint64_t strides[1] = { (cuuint64_t) t.pitch * (bytes ? 1 : 2) };
+    const cuuint64_t strides[1] = { (cuuint64_t) t.pitch * size };
     const cuuint32_t box[2] = { (cuuint32_t) box_inner, (cuuint32_t) box_rows };
     const cuuint32_t es[2] = { 1, 1 };
-    const CUtensorMapDataType type = bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                           : dtype == GLMX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUtensorMapDataType type = size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == GLMX_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const CUresult r = fn(m, type, 2, const_cast<void*>(t.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

@@ -24,6 +24,7 @@ struct Epi
 {
     int M, N;
     int bf16;                   // 16-bit type: bf16 or fp16
+    int tma;                    // pair_kernel: y is written by TMA (rows 16 bytes apart at least, nothing added)
     int vec;                    // rows of every output can take 16-byte stores (always but for I8 with an odd width)
     void* y; long long ldy; int y_dtype, accumulate;     // STORE, I8
     void* o0; void* o1;         // GATED: o0 = h; DACT: o0 = dg, o1 = du, [M][N]
@@ -32,24 +33,23 @@ struct Epi
     const float* xs; const float* ws; const float* bias; // I8
 };
 
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, int bf16)
+{
+    if (bf16)
+    {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&b);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <int W>
 __device__ __forceinline__ void store16(void* base, size_t off, const float (&v)[W], int bf16)
 {
     uint32_t w[W / 2];
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i)
-    {
-        if (bf16)
-        {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        else
-        {
-            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    }
+    for (int i = 0; i < W / 2; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], bf16);
     uint8_t* d = static_cast<uint8_t*>(base) + off * 2;
     *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
 }
@@ -275,6 +275,17 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
         : "memory");
 }
 
+// a tile of shared memory (128-byte swizzle) to global memory; rows and columns past the edges are left out
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n cp.async.bulk.commit_group;" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -292,6 +303,7 @@ constexpr int MAXPROB = 3;
 struct PairMaps
 {
     CUtensorMap a[MAXPROB], b[MAXPROB];
+    CUtensorMap y[MAXPROB];     // STORE, I8 with Epi.tma: boxes of 32 rows x 128 bytes
 };
 
 struct PairArgs
@@ -440,12 +452,64 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             find(t, p, m, n);
             if (!mbar_wait_bounded(&tfull[acc], (uint32_t) ((lt >> 1) & 1))) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
             tc_after();
-            const Epi& e = a.e[p];
+            const Epi e = a.e[p];       // in registers: the stores in between would have it read again
             const uint32_t tq = tmem + ((uint32_t) (32 * q) << 16) + (uint32_t) (acc * 256);
             // this warp's half of the tile's columns, 32 at a time (GATED: 16 of gate and of up): a lane holds a row, and through shared memory
             // each 8 (4) lanes get 4 columns each of one row, so that global accesses run along rows
             const int cols = EPI == EPI_GATED ? BN / 4 : BN / 2, c0 = half * cols;
             constexpr int CC = EPI == EPI_GATED ? 16 : 32, LPR = CC / 4;
+            if (EPI == EPI_STORE || EPI == EPI_I8)
+                if (e.tma)
+                {
+                    // whole rows of 128 bytes (64 or 32 columns) into the staging tile, from there by TMA
+                    const int row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
+                    const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
+                    const float xs = EPI == EPI_I8 && row0 + lane < e.M ? e.xs[row0 + lane] : 0.0f;
+                    const int wide = f32 ? 32 : 64;
+                    for (int c = c0; c < c0 + cols; c += wide)
+                    {
+                        const int n0 = n * BN + c;
+                        if (lane == 0) tma_store_read();                   // the tile before has been read
+                        __syncwarp();
+                        for (int d = 0; d < wide; d += 16)
+                        {
+                            uint32_t v[16];
+                            tc_ld16(tq + (uint32_t) (c + d), v);
+                            tc_wait_ld();
+                            if constexpr (EPI == EPI_I8)
+                            {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                {
+                                    const int col = min(n0 + d + i, e.N - 1);
+                                    float f = (float) (int) v[i] * (xs * __ldg(e.ws + col));
+                                    if (e.bias) f += __ldg(e.bias + col);
+                                    v[i] = __float_as_uint(f);
+                                }
+                            }
+                            if (f32)
+                            {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) stg[lane * 8 + ((d / 4 + i) ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                            }
+                            else
+                            {
+                                uint32_t w[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) w[i] = pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), bf);
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) stg[lane * 8 + ((d / 8 + i) ^ (lane & 7))] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0 && row0 < e.M && n0 < e.N) tma_store_2d(&maps.y[p], n0, row0, smem_u32(stg));
+                    }
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_remote(map_rank(smem_u32(&tempty[acc]), 0));
+                    continue;
+                }
             for (int c = c0; c < c0 + cols; c += CC)
             {
                 uint32_t v[16], u[16];
@@ -487,6 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             __syncwarp();
             if (lane == 0) arrive_remote(map_rank(smem_u32(&tempty[acc]), 0));
         }
+        if (lane == 0) tma_store_done();
     }
     __syncwarp();
     if (s_abort) drain_pause();
@@ -727,6 +792,13 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
     for (int i = 0; i < nprob; ++i)
     {
         a.e[i] = pr[i].e;
+        const Epi& e = pr[i].e;
+        if (EPI == EPI_STORE || EPI == EPI_I8)
+        {
+            a.e[i].tma = e.vec && !e.accumulate;
+            if (a.e[i].tma)
+                if ((err = dense_map(&maps.y[i], e.y_dtype, Mat{ e.y, e.M, e.N, e.ldy }, e.y_dtype == GLMX_F32 ? 32 : 64, 32)) != cudaSuccess) return err;
+        }
         a.mt[i] = (pr[i].e.M + 255) / 256;
         a.nt[i] = (pr[i].e.N + width - 1) / width;
         a.tile0[i + 1] = a.tile0[i] + a.mt[i] * a.nt[i];
