@@ -12,13 +12,6 @@ namespace glmx {
 
 namespace {
 
-template <bool W_MN, int EPI>
-cudaError_t product(int dtype, const Product& p, int nseg, int K, bool prefetch, cudaStream_t st)
-{
-    if (use_pair(p.e.M, false)) return launch_pair<false, false, W_MN, EPI>(dtype, 1, &p, nseg, K, 256, st);
-    return launch_cols<false, W_MN, EPI>(dtype, p, nseg, K, prefetch, st);
-}
-
 Epi epi(const glmx_ffn* f, int M, int N)
 {
     Epi e{};
@@ -66,7 +59,7 @@ extern "C" int glmx_ffn_forward(const glmx_ffn* f, const void* x, long long ldx,
     g.b[1] = { f->w_up, I, H, H };
     g.e = epi(f, ntok, I);
     g.e.o0 = h; g.e.p = p; g.e.q = q;
-    cudaError_t e = product<false, EPI_GATED>(f->dtype, g, 1, H, false, st);
+    cudaError_t e = launch_product<false, false, EPI_GATED>(f->dtype, g, 1, H, false, st);
     if (e == cudaSuccess)
     {
         Product d{};
@@ -76,7 +69,7 @@ extern "C" int glmx_ffn_forward(const glmx_ffn* f, const void* x, long long ldx,
         d.e.y = y; d.e.ldy = ldy; d.e.y_dtype = y_dtype; d.e.accumulate = accumulate;
         d.e.vec = ldy * (y_dtype == GLMX_F32 ? 4 : 2) % 16 == 0;
         // the kernel in front is this call's own and writes no weights: they may be read while it runs
-        e = product<false, EPI_STORE>(f->dtype, d, 1, I, true, st);
+        e = launch_product<false, false, EPI_STORE>(f->dtype, d, 1, I, true, st);
     }
     return e == cudaSuccess ? GLMX_OK : dense_cuda_fail(e, "glmx_ffn_forward: launch");
 }
@@ -114,7 +107,7 @@ extern "C" int glmx_ffn_backward(const glmx_ffn* f, const void* dy, long long ld
         d.b[0] = { f->w_down, H, I, I };
         d.e = epi(f, ntok, I);
         d.e.o0 = dg; d.e.o1 = du; d.e.p = const_cast<float*>(p); d.e.q = const_cast<float*>(q);
-        e = product<true, EPI_DACT>(f->dtype, d, 1, H, false, st);
+        e = launch_product<false, true, EPI_DACT>(f->dtype, d, 1, H, false, st);
     }
     if (e == cudaSuccess && dx)
     {
@@ -123,7 +116,7 @@ extern "C" int glmx_ffn_backward(const glmx_ffn* f, const void* dy, long long ld
         d.a[1] = { du, ntok, I, I }; d.b[1] = { f->w_up, I, H, H };
         d.e = epi(f, ntok, H);
         d.e.y = dx;
-        e = product<true, EPI_STORE>(f->dtype, d, 2, I, true, st);
+        e = launch_product<false, true, EPI_STORE>(f->dtype, d, 2, I, true, st);
     }
     Product w[3] = {};
     int n = 0;
@@ -136,6 +129,10 @@ extern "C" int glmx_ffn_backward(const glmx_ffn* f, const void* dy, long long ld
     if (dw_gate) add(dg, I, I, x, H, ldx, dw_gate);
     if (dw_up) add(du, I, I, x, H, ldx, dw_up);
     if (dw_down) add(dy, H, lddy, h, I, I, dw_down);
-    if (e == cudaSuccess && n) e = launch_pair<false, true, true, EPI_STORE>(f->dtype, n, w, 1, ntok, 256, st);
+    if (e == cudaSuccess && n)
+    {
+        const Epi es[3] = { w[0].e, w[1].e, w[2].e };
+        e = launch_pair<false, true, true, EPI_STORE>(f->dtype, n, w, 1, ntok, pair_plan(n, es, false, false, (ntok + 63) / 64, dense_sms(dense_device())).BN, st);
+    }
     return e == cudaSuccess ? GLMX_OK : dense_cuda_fail(e, "glmx_ffn_backward: launch");
 }

@@ -240,6 +240,15 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16])
         : "r"(taddr));
 }
 
+// one lane of a converged warp: issuing instructions under it, with the loops around them run by the whole warp, keeps
+// descriptors and addresses in uniform registers
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ uint32_t cluster_rank()
 {
     uint32_t r;
@@ -266,11 +275,11 @@ __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr)
 }
 
 // a CTA pair's load: into this CTA's shared memory, counted on a barrier that may be the other CTA's
-__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
 {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_u32(dst)),
+            dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
@@ -288,6 +297,40 @@ __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.w
 
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Bounded wait for a stage. The clock is first read after many tries: reading it takes longer than a stage does.
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity)
+{
+    for (int i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait_bounded(bar, parity);
+}
+
+// The same for a whole warp that waits long: one lane asks, with pauses. (256 threads that ask without one keep the shared-memory
+// pipe so busy that the loads' and MMAs' threads take twice as long for a stage.) False where the wait expired.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity)
+{
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0)
+    {
+        ok = false;
+        for (int i = 0; i < 64 && !(ok = mbar_try_wait(bar, parity)); ++i) __nanosleep(64);
+        if (!ok) ok = mbar_wait_bounded(bar, parity);
+    }
+    return __shfl_sync(0xffffffffu, (int) ok, 0) != 0;
+}
+
+// place in a ring of stages and the parity of its round
+struct Ring
+{
+    int s = 0, n;
+    uint32_t ph = 0;
+    __device__ __forceinline__ explicit Ring(int stages) : n(stages) {}
+    __device__ __forceinline__ void next()
+    {
+        if (++s == n) { s = 0; ph ^= 1u; }
+    }
+};
 
 // wait for asynchronous copies that nobody will wait for any more (only after a bounded wait has expired)
 __device__ __forceinline__ void drain_pause()
@@ -311,7 +354,7 @@ struct PairArgs
     int nprob;                  // products in the launch (the weights' gradients: three); problem p has maps a[p], b[p], epilogue e[p]
     int nseg;                   // 1; 2: one product whose sum runs over a[0] b[0] and a[1] b[1]
     int K, bk;                  // inputs per segment, and per stage (128 bytes)
-    int BN;                     // columns per tile: 128 or 256
+    int BN;                     // columns per tile: 64 (weights K-major only), 128 or 256
     int mt[MAXPROB], nt[MAXPROB], tile0[MAXPROB + 1];    // tiles along M and N, and the first tile of each problem
     uint32_t idesc;
     int* err;
@@ -342,7 +385,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_abort;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int BN = a.BN, NST = pair_stages(BN), STAGE = pair_stage(BN);
     if (tid == 0)
@@ -373,70 +416,85 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
     if (warp == 0)
     {
-        if (lane == 0)
+        // (this loop and the MMA's run a stage in few instructions, without divisions: at 256 columns a stage takes about 500 cycles)
+        Ring r(NST);
+        const uint32_t full0 = map_rank(smem_u32(&full[0]), 0), smem0 = smem_u32(smem), bytes = (uint32_t) (2 * STAGE);
+        const int bk = a.bk, nseg = a.nseg;
+        for (int t = first; t < ntiles && !s_abort; t += pairs)
         {
-            int it = 0;
-            for (int t = first; t < ntiles && !s_abort; t += pairs)
+            int p, m, n;
+            find(t, p, m, n);
+            const int m0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM;
+            const int n0 = EPI == EPI_GATED ? n * (BN / 2) : n * BN + (int) rank * (BN / 2);
+            for (int seg = 0; seg < nseg && !s_abort; ++seg)
             {
-                int p, m, n;
-                find(t, p, m, n);
-                for (int k = 0; k < nk; ++k, ++it)
+                const int mp = nseg > 1 ? seg : p;
+                const CUtensorMap* ma = &maps.a[mp];
+                // GATED: gate columns from CTA 0, the same up columns from CTA 1
+                const CUtensorMap* mb = &maps.b[EPI == EPI_GATED ? (int) rank : mp];
+                for (int k = 0, kc = 0; k < ksteps; ++k, kc += bk)
                 {
-                    const int s = it % NST;
-                    if (!mbar_wait_bounded(&empty[s], (uint32_t) ((it / NST) & 1) ^ 1u)) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
-                    const int seg = k / ksteps, kc = (k - seg * ksteps) * a.bk, mp = a.nseg > 1 ? seg : p;
-                    uint8_t* sa = smem + (size_t) s * STAGE;
-                    uint8_t* sb = sa + PAIR_BM * 128;
-                    // the pair's four half tiles are counted on the leader's barrier
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t) (2 * STAGE));
-                    const uint32_t bar = map_rank(smem_u32(&full[s]), 0);
-                    const int m0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM;
-                    if constexpr (A_MN)
-                        for (int j = 0; j < 2; ++j) tma_load_pair(sa + j * 8192, &maps.a[mp], m0 + 64 * j, kc, bar);
-                    else
-                        tma_load_pair(sa, &maps.a[mp], kc, m0, bar);
-                    if constexpr (EPI == EPI_GATED)
-                        // gate columns from CTA 0, the same up columns from CTA 1
-                        tma_load_pair(sb, &maps.b[rank], kc, n * (BN / 2), bar);
-                    else
+                    if (!ring_wait(&empty[r.s], r.ph ^ 1u)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
+                    const uint32_t sa = smem0 + (uint32_t) (r.s * STAGE), sb = sa + PAIR_BM * 128, bar = full0 + 8u * r.s;
+                    if (elect_one())
                     {
-                        const int n0 = n * BN + (int) rank * (BN / 2);
-                        if constexpr (B_MN)
-                            for (int j = 0; j < BN / 128; ++j) tma_load_pair(sb + j * 8192, &maps.b[mp], n0 + 64 * j, kc, bar);
+                        // the pair's four half tiles are counted on the leader's barrier
+                        if (rank == 0) mbar_arrive_expect_tx(&full[r.s], bytes);
+                        if constexpr (A_MN)
+                        {
+                            tma_load_pair(sa, ma, m0, kc, bar);
+                            tma_load_pair(sa + 8192, ma, m0 + 64, kc, bar);
+                        }
                         else
-                            tma_load_pair(sb, &maps.b[mp], kc, n0, bar);
+                            tma_load_pair(sa, ma, kc, m0, bar);
+                        if constexpr (B_MN)
+                        {
+                            tma_load_pair(sb, mb, n0, kc, bar);
+                            if (BN > 128) tma_load_pair(sb + 8192, mb, n0 + 64, kc, bar);
+                        }
+                        else
+                            tma_load_pair(sb, mb, kc, n0, bar);
                     }
+                    __syncwarp();
+                    r.next();
                 }
             }
-            // the last arrivals on this CTA's barriers come from the pair's leader: they are in before it may exit
-            for (int i = it > NST ? it - NST : 0; i < it && !s_abort; ++i)
-                if (!mbar_wait_bounded(&empty[i % NST], (uint32_t) ((i / NST) & 1))) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; }
         }
+        // the last arrivals on this CTA's barriers come from the pair's leader: they are in before it may exit
+        for (int i = 0; i < NST && !s_abort; ++i, r.next())
+            if (!ring_wait(&empty[r.s], r.ph ^ 1u)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; }
     }
     else if (warp == 1)
     {
-        if (lane == 0 && rank == 0)
+        if (rank == 0)
         {
-            int it = 0, lt = 0;
+            Ring r(NST);
+            int lt = 0;
+            const uint64_t da0 = desc_sw128(smem_u32(smem), 8192), db0 = desc_sw128(smem_u32(smem) + PAIR_BM * 128, 8192);
+            const uint32_t idesc = a.idesc;
             for (int t = first; t < ntiles && !s_abort; t += pairs, ++lt)
             {
                 const int acc = lt & 1;
-                if (!mbar_wait_bounded(&tempty[acc], (uint32_t) ((lt >> 1) & 1) ^ 1u)) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
+                const uint32_t d = tmem + (uint32_t) (acc * 256);
+                if (!ring_wait(&tempty[acc], (uint32_t) ((lt >> 1) & 1) ^ 1u)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
                 tc_after();
-                for (int k = 0; k < nk; ++k, ++it)
+                for (int k = 0; k < nk; ++k)
                 {
-                    const int s = it % NST;
-                    if (!mbar_wait_bounded(&full[s], (uint32_t) ((it / NST) & 1))) { atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
+                    if (!ring_wait(&full[r.s], r.ph)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
                     tc_after();
-                    const uint32_t sa = smem_u32(smem + (size_t) s * STAGE), sb = sa + PAIR_BM * 128;
+                    // descriptors count 16-byte units: a stage, and 32 bytes of K (16 rows of an MN-major tile) per instruction
+                    const uint64_t off = (uint64_t) (uint32_t) (r.s * STAGE >> 4);
+                    if (elect_one())
+                    {
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        tc_mma<I8, 2>(tmem + (uint32_t) (acc * 256), desc_sw128(sa + kk * (A_MN ? 2048 : 32), 8192),
-                                      desc_sw128(sb + kk * (B_MN ? 2048 : 32), 8192), a.idesc, (k | kk) != 0);
-                    tc_commit<2>(&empty[s]);
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma<I8, 2>(d, da0 + off + kk * (A_MN ? 128 : 2), db0 + off + kk * (B_MN ? 128 : 2), idesc, (k | kk) != 0);
+                        tc_commit<2>(&empty[r.s]);
+                        if (k == nk - 1) tc_commit<2>(&tfull[acc]);
+                    }
+                    __syncwarp();
+                    r.next();
                 }
-                if (s_abort) break;
-                tc_commit<2>(&tfull[acc]);
             }
         }
     }
@@ -450,7 +508,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             const int acc = lt & 1;
             int p, m, n;
             find(t, p, m, n);
-            if (!mbar_wait_bounded(&tfull[acc], (uint32_t) ((lt >> 1) & 1))) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
+            if (!warp_wait(&tfull[acc], (uint32_t) ((lt >> 1) & 1))) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
             tc_after();
             const Epi e = a.e[p];       // in registers: the stores in between would have it read again
             const uint32_t tq = tmem + ((uint32_t) (32 * q) << 16) + (uint32_t) (acc * 256);
@@ -465,8 +523,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     const int row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
                     const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
                     const float xs = EPI == EPI_I8 && row0 + lane < e.M ? e.xs[row0 + lane] : 0.0f;
-                    const int wide = f32 ? 32 : 64;
-                    for (int c = c0; c < c0 + cols; c += wide)
+                    const int wide = f32 ? 32 : 64, share = max(wide, BN / 2);   // (of a narrow tile, one warp takes all columns)
+                    for (int c = half * share; c < min(BN, (half + 1) * share); c += wide)
                     {
                         const int n0 = n * BN + c;
                         if (lane == 0) tma_store_read();                   // the tile before has been read
@@ -598,28 +656,31 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_abort;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int splits = gridDim.x, split = blockIdx.x;      // one cluster along x
     const int mtile = blockIdx.y % a.mtiles, ttile = blockIdx.y / a.mtiles;
     const int NT = a.NT, NST = a.stages, STAGE = 16384 + NT * 128;
     const int ksteps = (a.K + a.bk - 1) / a.bk, nk_all = ksteps * a.nseg;
     const int k0 = (int) ((long long) nk_all * split / splits), nk = (int) ((long long) nk_all * (split + 1) / splits) - k0;
     const int rows = EPI == EPI_GATED ? 64 : 128;          // output columns (weight rows of one matrix) per tile
-    auto load_w = [&](int i) {
-        const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
+    // next stage to load: segment and place in it
+    int seg = k0 / ksteps, kc = (k0 - seg * ksteps) * a.bk;
+    const int kend = ksteps * a.bk;
+    auto step = [&](int& sg, int& c) {
+        c += a.bk;
+        if (c == kend) { c = 0; ++sg; }
+    };
+    auto load_w = [&](int s, int sg, int c) {
         uint8_t* sw = smem + (size_t) s * STAGE;
         mbar_arrive_expect_tx(&full[s], (uint32_t) STAGE);
         if constexpr (EPI == EPI_GATED)
-            for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[j], kc, mtile * 64, &full[s]);
+            for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[j], c, mtile * 64, &full[s]);
         else if constexpr (W_MN)
-            for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[seg], mtile * 128 + 64 * j, kc, &full[s]);
+            for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[sg], mtile * 128 + 64 * j, c, &full[s]);
         else
-            tma_load_2d(sw, &maps.w[seg], kc, mtile * 128, &full[s]);
+            tma_load_2d(sw, &maps.w[sg], c, mtile * 128, &full[s]);
     };
-    auto load_x = [&](int i) {
-        const int s = i % NST, k = k0 + i, seg = k / ksteps, kc = (k - seg * ksteps) * a.bk;
-        tma_load_2d(smem + (size_t) s * STAGE + 16384, &maps.x[seg], kc, ttile * NT, &full[s]);
-    };
+    auto load_x = [&](int s, int sg, int c) { tma_load_2d(smem + (size_t) s * STAGE + 16384, &maps.x[sg], c, ttile * NT, &full[s]); };
     const int ahead = nk < NST ? nk : NST;                 // stages that need no wait
     if (tid == 0)
     {
@@ -629,9 +690,9 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
         fence_barrier_init();
         // the first loads do not wait for the rest of the CTA
         if (!a.prefetch) grid_wait();
-        for (int i = 0; i < ahead; ++i) load_w(i);
+        for (int i = 0, sg = seg, c = kc; i < ahead; ++i, step(sg, c)) load_w(i, sg, c);
         if (a.prefetch) grid_wait();
-        for (int i = 0; i < ahead; ++i) load_x(i);
+        for (int i = 0; i < ahead; ++i, step(seg, kc)) load_x(i, seg, kc);
     }
     if (warp == 1) tc_alloc<1>(&tmem_slot, (uint32_t) a.tcols);
     __syncwarp();
@@ -643,40 +704,47 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
 
     if (warp == 0)
     {
-        if (lane == 0)
+        // lane 0's segment and place after the first loads
+        seg = __shfl_sync(0xffffffffu, seg, 0);
+        kc = __shfl_sync(0xffffffffu, kc, 0);
+        Ring r(NST);
+        r.ph = 1;                                          // the ring's second round
+        for (int i = ahead; i < nk; ++i, step(seg, kc), r.next())
         {
-            for (int i = ahead; i < nk; ++i)
+            if (!ring_wait(&empty[r.s], r.ph ^ 1u)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
+            if (elect_one())
             {
-                const int s = i % NST;
-                if (!mbar_wait_bounded(&empty[s], (uint32_t) ((i / NST) & 1) ^ 1u)) { atomicOr(a.err, ERR_TIMEOUT_EMPTY); s_abort = 1; break; }
-                load_w(i);
-                load_x(i);
+                load_w(r.s, seg, kc);
+                load_x(r.s, seg, kc);
             }
+            __syncwarp();
         }
     }
     else if (warp == 1)
     {
         grid_wait();
-        if (lane == 0)
+        Ring r(NST);
+        const uint64_t dw0 = desc_sw128(smem_u32(smem), 8192), dx0 = desc_sw128(smem_u32(smem) + 16384, 8192);
+        const uint32_t idesc = a.idesc;
+        for (int i = 0; i < nk; ++i, r.next())
         {
-            for (int i = 0; i < nk; ++i)
+            if (!ring_wait(&full[r.s], r.ph)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
+            tc_after();
+            const uint64_t off = (uint64_t) (uint32_t) (r.s * STAGE >> 4);
+            if (elect_one())
             {
-                const int s = i % NST;
-                if (!mbar_wait_bounded(&full[s], (uint32_t) ((i / NST) & 1))) { atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; break; }
-                tc_after();
-                const uint32_t sw = smem_u32(smem + (size_t) s * STAGE), sx = sw + 16384;
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    tc_mma<I8, 1>(tmem, desc_sw128(sw + kk * (W_MN ? 2048 : 32), 8192), desc_sw128(sx + kk * 32, 8192), a.idesc, (i | kk) != 0);
-                tc_commit<1>(&empty[s]);
+                for (int kk = 0; kk < 4; ++kk) tc_mma<I8, 1>(tmem, dw0 + off + kk * (W_MN ? 128 : 2), dx0 + off + kk * 2, idesc, (i | kk) != 0);
+                tc_commit<1>(&empty[r.s]);
+                if (i == nk - 1) tc_commit<1>(&tfull);
             }
-            tc_commit<1>(&tfull);
+            __syncwarp();
         }
     }
     __syncwarp();
     grid_wait();
     // every load has been multiplied: the partial tile [token][weight row] takes the ring's place
-    if (!mbar_wait_bounded(&tfull, 0)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; }
+    if (warp >= 2 && !warp_wait(&tfull, 0)) { if (lane == 0) atomicOr(a.err, ERR_TIMEOUT_FULL); s_abort = 1; }
     if (s_abort) drain_pause();
     __syncthreads();
     tc_after();
@@ -817,28 +885,71 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
     return launch_chained(kernel, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), (size_t) pair_smem(BN), st, maps, a);
 }
 
+// Seconds of a launch, in microseconds, by a simple model of what was measured on a B200; the kernel and its tiling are those of the least.
+//   pair_kernel: rounds of tiles over the pairs, each stage (128 bytes of K) 0.46 us at 256 columns, 0.29 at 128, 0.21 at 64
+//     (the loads of A then bind), plus 1.5 us per round to fill the ring and drain a tile, plus 4.
+//   cols_kernel: rounds of clusters, each CTA 4 us (start, join) plus its stages; a stage takes its share of the weights'
+//     stream from memory, or the tensor cores' and L2's time for its tokens.
+struct PairPlan
+{
+    int BN;
+    double us;
+};
+
+inline PairPlan pair_plan(int nprob, const Epi* e, bool gated, bool narrow_ok, int nk, int sms)
+{
+    PairPlan best{ 256, 1e30 };
+    for (int BN = 256; BN >= (narrow_ok ? 64 : 128); BN /= 2)
+    {
+        long long tiles = 0;
+        const int width = gated ? BN / 2 : BN;
+        for (int i = 0; i < nprob; ++i) tiles += (long long) ((e[i].M + 255) / 256) * ((e[i].N + width - 1) / width);
+        const double rounds = (double) ((tiles + sms / 2 - 1) / (sms / 2));
+        const double us = 4.0 + rounds * (1.5 + nk * (BN == 256 ? 0.46 : BN == 128 ? 0.29 : 0.21));
+        if (us < best.us - 1e-9) best = { BN, us };
+    }
+    return best;
+}
+
 struct ColsPlan
 {
     int NT, ttiles, mtiles, splits, stages;
+    double us;
 };
 
-// Tokens per tile: all of them up to 256, else equal tiles. Splits of K: the count (at most 8, the portable cluster size) that
-// leaves the SMs the fewest rounds of the least work, each CTA with at least two stages.
-inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms)
+constexpr int COLS_SMEM2 = 112 * 1024, COLS_SMEM1 = 224 * 1024;   // two CTAs an SM (tiles of up to 64 tokens), or one
+
+// clusters of each size that the device holds at once, for either shared memory size
+struct ColsCapacity
+{
+    int n[2][9];
+};
+
+// Tokens per tile: all of them up to 256, else equal tiles. Splits of K: at most 8 (the portable cluster size), each CTA with at least
+// two stages.
+inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms, const ColsCapacity& cap)
 {
     ColsPlan p;
     p.ttiles = (M + 255) / 256;
     p.NT = ((M + p.ttiles - 1) / p.ttiles + 15) / 16 * 16;
     p.mtiles = (N + (gated ? 63 : 127)) / (gated ? 64 : 128);
-    const int stage = 16384 + p.NT * 128, tiles = p.ttiles * p.mtiles;
+    const int stage = 16384 + p.NT * 128, one = p.NT <= 64 ? 0 : 1;
+    const long long tiles = (long long) p.ttiles * p.mtiles;
     p.splits = 1;
-    double best = 1e30;
+    p.us = 1e30;
     for (int s = 1; s <= 8 && (s == 1 || 2 * s <= nk); ++s)
     {
-        const double rounds = (double) ((tiles * s + sms - 1) / sms), cost = rounds * ((nk + s - 1) / s + 2.0);
-        if (cost < best - 1e-9) { best = cost; p.splits = s; }
+        const int room = cap.n[one][s];
+        if (room < 1) continue;
+        const long long rounds = (tiles + room - 1) / room;
+        const double ctas = (double) (tiles < room ? tiles : room) * s;              // running at once
+        const double stream = ctas * 16384 / 5.5e6, l2 = ctas * stage / 9.0e6, mma = 0.2 + p.NT * 0.0016;
+        const double step = (stream > l2 ? stream : l2) > mma ? (stream > l2 ? stream : l2) : mma;
+        const double us = rounds * (4.0 + (double) ((nk + s - 1) / s) * step);
+        if (us < p.us - 1e-9) { p.us = us; p.splits = s; }
     }
-    const int room = p.NT <= 64 ? 112 * 1024 : 224 * 1024, per = (nk + p.splits - 1) / p.splits;
+    (void) sms;
+    const int room = one ? COLS_SMEM1 : COLS_SMEM2, per = (nk + p.splits - 1) / p.splits;
     p.stages = (room - 2048) / stage;
     if (p.stages > COLS_STAGES_MAX) p.stages = COLS_STAGES_MAX;
     const int part = (p.NT * 512 + stage - 1) / stage;     // the partial tile takes the ring's place
@@ -848,22 +959,43 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms)
 }
 
 template <bool I8, bool W_MN, int EPI>
-cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, bool prefetch, cudaStream_t st)
+cudaError_t cols_capacity(int dev, const ColsCapacity** out)
 {
     auto kernel = cols_kernel<I8, W_MN, EPI>;
-    const int dev = dense_device();
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    static ColsCapacity cap[64] = {};
     static bool ready[64] = {};
-    cudaError_t err;
     if (!ready[dev])
     {
-        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024)) != cudaSuccess) return err;
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, COLS_SMEM1);
+        for (int i = 0; i < 2; ++i)
+            for (int s = 1; s <= 8 && err == cudaSuccess; ++s)
+            {
+                cudaLaunchConfig_t cfg = {};
+                cfg.gridDim = dim3(s, 1024);
+                cfg.blockDim = dim3(COLS_THREADS);
+                cfg.dynamicSmemBytes = i ? COLS_SMEM1 : COLS_SMEM2;
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeClusterDimension;
+                attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+                cfg.attrs = attr;
+                cfg.numAttrs = 1;
+                err = cudaOccupancyMaxActiveClusters(&cap[dev].n[i][s], kernel, &cfg);
+            }
+        if (err != cudaSuccess) return err;
         ready[dev] = true;
     }
+    *out = &cap[dev];
+    return cudaSuccess;
+}
+
+template <bool I8, bool W_MN, int EPI>
+cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, const ColsPlan& p, bool prefetch, cudaStream_t st)
+{
+    auto kernel = cols_kernel<I8, W_MN, EPI>;
+    cudaError_t err;
     ColsMaps maps;
     ColsArgs a{};
     a.nseg = nseg; a.K = K; a.bk = I8 ? 128 : 64;
-    const ColsPlan p = cols_plan(pr.e.M, pr.e.N, EPI == EPI_GATED, nseg * ((K + a.bk - 1) / a.bk), dense_sms(dev));
     a.NT = p.NT; a.stages = p.stages; a.mtiles = p.mtiles; a.prefetch = prefetch;
     a.tcols = 32;
     while (a.tcols < p.NT) a.tcols *= 2;
@@ -889,8 +1021,20 @@ cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, bool pref
     return cudaLaunchKernelEx(&cfg, kernel, maps, a);
 }
 
-// Which kernel: few rows go to cols_kernel, many to pair_kernel. Measured (us, cols / pair): feed-forward of 256 rows at
-// H = 6144, I = 1536 62 / 63 and of 512 rows 91 / 64; int8 product of 48 rows at K = N = 6144 13 / 31, of 256 rows 40 / 33.
-inline bool use_pair(int M, bool i8) { return M > (i8 ? 160 : 384); }
+// One product by the kernel and tiling of the least modelled time.
+template <bool I8, bool W_MN, int EPI>
+cudaError_t launch_product(int dtype, const Product& pr, int nseg, int K, bool prefetch, cudaStream_t st)
+{
+    const int dev = dense_device();
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    const int nk = nseg * ((K + (I8 ? 127 : 63)) / (I8 ? 128 : 64)), sms = dense_sms(dev);
+    const ColsCapacity* cap;
+    const cudaError_t err = cols_capacity<I8, W_MN, EPI>(dev, &cap);
+    if (err != cudaSuccess) return err;
+    const ColsPlan c = cols_plan(pr.e.M, pr.e.N, EPI == EPI_GATED, nk, sms, *cap);
+    const PairPlan p = pair_plan(1, &pr.e, EPI == EPI_GATED, !W_MN, nk, sms);
+    if (c.us <= p.us) return launch_cols<I8, W_MN, EPI>(dtype, pr, nseg, K, c, prefetch, st);
+    return launch_pair<I8, false, W_MN, EPI>(dtype, 1, &pr, nseg, K, p.BN, st);
+}
 
 }  // namespace glmx

@@ -75,7 +75,6 @@ extern "C" int glmx_linear_i8(const signed char* xq, long long ldxq, const float
     p.e.M = ntok; p.e.N = N; p.e.y = y; p.e.ldy = ldy; p.e.y_dtype = y_dtype;
     p.e.xs = x_scale; p.e.ws = w_scale; p.e.bias = bias;
     p.e.vec = dense_aligned(y) && ldy * (y_dtype == GLMX_F32 ? 4 : 2) % 16 == 0;
-    const cudaError_t e = use_pair(ntok, true) ? launch_pair<true, false, false, EPI_I8>(GLMX_I32, 1, &p, 1, K, 256, st)
-                                                        : launch_cols<true, false, EPI_I8>(GLMX_I32, p, 1, K, false, st);
+    const cudaError_t e = launch_product<true, false, EPI_I8>(GLMX_I32, p, 1, K, false, st);
     return e == cudaSuccess ? GLMX_OK : dense_cuda_fail(e, "glmx_linear_i8: launch");
 }
