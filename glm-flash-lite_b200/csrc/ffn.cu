@@ -12,6 +12,9 @@ namespace glmx {
 
 namespace {
 
+// rows of h, dg and du: 128-byte lines, which a copy of 128-byte boxes from rows between lines would read twice
+long long hidden_pitch(const glmx_ffn* f) { return (f->intermediate + 63) / 64 * 64; }
+
 Epi epi(const glmx_ffn* f, int M, int N)
 {
     Epi e{};
@@ -44,6 +47,7 @@ extern "C" int glmx_ffn_forward(const glmx_ffn* f, const void* x, long long ldx,
     int rc = check_ffn(f);
     if (rc) return rc;
     const int H = f->hidden, I = f->intermediate;
+    const long long P = hidden_pitch(f);
     if (ntok < 0) return dense_fail(GLMX_E_ARG, "glmx_ffn_forward: ntok >= 0 required");
     if (y_dtype != f->dtype && y_dtype != GLMX_F32) return dense_fail(GLMX_E_ARG, "glmx_ffn_forward: y must have the block's dtype or fp32");
     if (ldx < H || ldx % 8 || ldy < H) return dense_fail(GLMX_E_ARG, "glmx_ffn_forward: ldx must be a multiple of 8 and ldx, ldy >= hidden");
@@ -58,12 +62,12 @@ extern "C" int glmx_ffn_forward(const glmx_ffn* f, const void* x, long long ldx,
     g.b[0] = { f->w_gate, I, H, H };
     g.b[1] = { f->w_up, I, H, H };
     g.e = epi(f, ntok, I);
-    g.e.o0 = h; g.e.p = p; g.e.q = q;
+    g.e.o0 = h; g.e.ldo = P; g.e.p = p; g.e.q = q;
     cudaError_t e = launch_product<false, false, EPI_GATED>(f->dtype, g, 1, H, false, st);
     if (e == cudaSuccess)
     {
         Product d{};
-        d.a[0] = { h, ntok, I, I };
+        d.a[0] = { h, ntok, I, P };
         d.b[0] = { f->w_down, H, I, I };
         d.e = epi(f, ntok, H);
         d.e.y = y; d.e.ldy = ldy; d.e.y_dtype = y_dtype; d.e.accumulate = accumulate;
@@ -81,6 +85,7 @@ extern "C" int glmx_ffn_backward(const glmx_ffn* f, const void* dy, long long ld
     int rc = check_ffn(f);
     if (rc) return rc;
     const int H = f->hidden, I = f->intermediate;
+    const long long P = hidden_pitch(f);
     if (ntok < 0) return dense_fail(GLMX_E_ARG, "glmx_ffn_backward: ntok >= 0 required");
     if (lddy < H || lddy % 8 || ldx < H || ldx % 8)
         return dense_fail(GLMX_E_ARG, "glmx_ffn_backward: lddy and ldx must be multiples of 8, at least hidden");
@@ -106,14 +111,14 @@ extern "C" int glmx_ffn_backward(const glmx_ffn* f, const void* dy, long long ld
         d.a[0] = { dy, ntok, H, lddy };
         d.b[0] = { f->w_down, H, I, I };
         d.e = epi(f, ntok, I);
-        d.e.o0 = dg; d.e.o1 = du; d.e.p = const_cast<float*>(p); d.e.q = const_cast<float*>(q);
+        d.e.o0 = dg; d.e.o1 = du; d.e.ldo = P; d.e.p = const_cast<float*>(p); d.e.q = const_cast<float*>(q);
         e = launch_product<false, true, EPI_DACT>(f->dtype, d, 1, H, false, st);
     }
     if (e == cudaSuccess && dx)
     {
         Product d{};
-        d.a[0] = { dg, ntok, I, I }; d.b[0] = { f->w_gate, I, H, H };
-        d.a[1] = { du, ntok, I, I }; d.b[1] = { f->w_up, I, H, H };
+        d.a[0] = { dg, ntok, I, P }; d.b[0] = { f->w_gate, I, H, H };
+        d.a[1] = { du, ntok, I, P }; d.b[1] = { f->w_up, I, H, H };
         d.e = epi(f, ntok, H);
         d.e.y = dx;
         e = launch_product<false, true, EPI_STORE>(f->dtype, d, 2, I, true, st);
@@ -126,9 +131,9 @@ extern "C" int glmx_ffn_backward(const glmx_ffn* f, const void* dy, long long ld
         w[n].e = epi(f, (int) width, N);
         w[n++].e.y = out;
     };
-    if (dw_gate) add(dg, I, I, x, H, ldx, dw_gate);
-    if (dw_up) add(du, I, I, x, H, ldx, dw_up);
-    if (dw_down) add(dy, H, lddy, h, I, I, dw_down);
+    if (dw_gate) add(dg, I, P, x, H, ldx, dw_gate);
+    if (dw_up) add(du, I, P, x, H, ldx, dw_up);
+    if (dw_down) add(dy, H, lddy, h, I, P, dw_down);
     if (e == cudaSuccess && n)
     {
         const Epi es[3] = { w[0].e, w[1].e, w[2].e };

@@ -24,11 +24,11 @@ struct Epi
 {
     int M, N;
     int bf16;                   // 16-bit type: bf16 or fp16
-    int tma;                    // pair_kernel: y is written by TMA (rows 16 bytes apart at least, nothing added)
     int vec;                    // rows of every output can take 16-byte stores (always but for I8 with an odd width)
     void* y; long long ldy; int y_dtype, accumulate;     // STORE, I8
-    void* o0; void* o1;         // GATED: o0 = h; DACT: o0 = dg, o1 = du, [M][N]
-    float* p; float* q;
+    void* o0; void* o1;         // GATED: o0 = h; DACT: o0 = dg, o1 = du; [M] rows of N, ldo apart
+    long long ldo;
+    float* p; float* q;         // [M][N]
     float limit;
     const float* xs; const float* ws; const float* bias; // I8
 };
@@ -92,7 +92,7 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
             pp[i] = ku ? act : 0.0f;
             qq[i] = kg ? up * (s + (g < -100.0f ? 0.0f : g * s * (1.0f - s))) : 0.0f;
         }
-        store16<W>(e.o0, o, hh, e.bf16);
+        store16<W>(e.o0, (size_t) t * e.ldo + n, hh, e.bf16);
         if (e.p) { store_f32<W>(e.p + o, pp); store_f32<W>(e.q + o, qq); }
         return;
     }
@@ -113,8 +113,8 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
                 du[4 * i + j] = d * pv[j];
             }
         }
-        store16<W>(e.o0, o, dg, e.bf16);
-        store16<W>(e.o1, o, du, e.bf16);
+        store16<W>(e.o0, (size_t) t * e.ldo + n, dg, e.bf16);
+        store16<W>(e.o1, (size_t) t * e.ldo + n, du, e.bf16);
         return;
     }
     if constexpr (EPI == EPI_I8)
@@ -339,6 +339,32 @@ __device__ __forceinline__ void drain_pause()
     while (globaltimer() - t0 < 1000000) __nanosleep(10000);
 }
 
+// A warp copies its staging tile (32 rows of 128 bytes, 16-byte piece i of row r at place i ^ (r & 7)) to rows of any alignment: fp32 by single
+// elements, 16-bit ones by words, which in rows that start between two words are made of neighbours' halves.
+__device__ __forceinline__ void copy_rows(const Epi& e, const uint4* stg, int row0, int n0, int wide, int lane)
+{
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(stg);
+    const int rows = min(32, e.M - row0), cols = min(wide, e.N - n0);
+    if (cols <= 0) return;
+    for (int r = 0; r < rows; ++r)
+    {
+        const uint32_t v = w[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4 + (lane & 3)];
+        if (wide == 32)
+        {
+            if (lane < cols) static_cast<uint32_t*>(e.y)[(size_t) (row0 + r) * e.ldy + n0 + lane] = v;
+            continue;
+        }
+        uint16_t* d = static_cast<uint16_t*>(e.y) + (size_t) (row0 + r) * e.ldy + n0;
+        const bool odd = (reinterpret_cast<uintptr_t>(d) & 2) != 0;
+        const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
+        const uint32_t word = odd ? (v >> 16) | (next << 16) : v;
+        const int c = 2 * lane + odd;                      // the word's first column
+        if (c + 1 < cols) *reinterpret_cast<uint32_t*>(d + c) = word;
+        else if (c < cols) d[c] = (uint16_t) word;
+        if (odd && lane == 0) d[0] = (uint16_t) v;
+    }
+}
+
 // ---- pair_kernel -------------------------------------------------------------------------------------------------------
 
 constexpr int MAXPROB = 3;
@@ -516,10 +542,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             // each 8 (4) lanes get 4 columns each of one row, so that global accesses run along rows
             const int cols = EPI == EPI_GATED ? BN / 4 : BN / 2, c0 = half * cols;
             constexpr int CC = EPI == EPI_GATED ? 16 : 32, LPR = CC / 4;
-            if (EPI == EPI_STORE || EPI == EPI_I8)
-                if (e.tma)
+            if (EPI == EPI_I8 || (EPI == EPI_STORE && !e.accumulate))
                 {
-                    // whole rows of 128 bytes (64 or 32 columns) into the staging tile, from there by TMA
+                    // whole rows of 128 bytes (64 or 32 columns) into the staging tile, from there by TMA, or row by row where the
+                    // output's rows are not 16-byte aligned
                     const int row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
                     const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
                     const float xs = EPI == EPI_I8 && row0 + lane < e.M ? e.xs[row0 + lane] : 0.0f;
@@ -561,7 +587,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0 && row0 < e.M && n0 < e.N) tma_store_2d(&maps.y[p], n0, row0, smem_u32(stg));
+                        if (!e.vec)
+                        {
+                            copy_rows(e, stg, row0, n0, wide, lane);
+                            __syncwarp();
+                        }
+                        else if (lane == 0 && row0 < e.M && n0 < e.N) tma_store_2d(&maps.y[p], n0, row0, smem_u32(stg));
                     }
                     tc_before();
                     __syncwarp();
@@ -583,25 +614,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 }
                 __syncwarp();
                 const int nn = n * (EPI == EPI_GATED ? BN / 2 : BN) + c, row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
-                if (EPI != EPI_I8 || e.vec)
-                {
 #pragma unroll
-                    for (int i = 0; i < LPR; ++i)
-                    {
-                        const int r = i * (32 / LPR) + lane / LPR, pc = lane % LPR;
-                        const uint4 x = stg[r * 8 + (pc ^ (r & 7))], y = EPI == EPI_GATED ? stg[r * 8 + ((pc + 4) ^ (r & 7))] : x;
-                        const uint32_t x4[4] = { x.x, x.y, x.z, x.w }, y4[4] = { y.x, y.y, y.z, y.w };
-                        emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4, y4);
-                    }
-                }
-                else
+                for (int i = 0; i < LPR; ++i)
                 {
-                    // rows that no wide store fits: a lane a column
-                    for (int r = 0; r < 32; ++r)
-                    {
-                        const uint32_t x1[1] = { reinterpret_cast<const uint32_t*>(stg)[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4 + (lane & 3)] };
-                        emit<EPI, 1>(e, row0 + r, nn + lane, x1, x1);
-                    }
+                    const int r = i * (32 / LPR) + lane / LPR, pc = lane % LPR;
+                    const uint4 x = stg[r * 8 + (pc ^ (r & 7))], y = EPI == EPI_GATED ? stg[r * 8 + ((pc + 4) ^ (r & 7))] : x;
+                    const uint32_t x4[4] = { x.x, x.y, x.z, x.w }, y4[4] = { y.x, y.y, y.z, y.w };
+                    emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4, y4);
                 }
                 __syncwarp();
             }
@@ -863,8 +882,7 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
         const Epi& e = pr[i].e;
         if (EPI == EPI_STORE || EPI == EPI_I8)
         {
-            a.e[i].tma = e.vec && !e.accumulate;
-            if (a.e[i].tma)
+            if (e.vec && !e.accumulate)
                 if ((err = dense_map(&maps.y[i], e.y_dtype, Mat{ e.y, e.M, e.N, e.ldy }, e.y_dtype == GLMX_F32 ? 32 : 64, 32)) != cudaSuccess) return err;
         }
         a.mt[i] = (pr[i].e.M + 255) / 256;
@@ -886,8 +904,8 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
 }
 
 // Seconds of a launch, in microseconds, by a simple model of what was measured on a B200; the kernel and its tiling are those of the least.
-//   pair_kernel: rounds of tiles over the pairs, each stage (128 bytes of K) 0.46 us at 256 columns, 0.29 at 128, 0.21 at 64
-//     (the loads of A then bind), plus 1.5 us per round to fill the ring and drain a tile, plus 4.
+//   pair_kernel: rounds of tiles over the pairs, each stage (128 bytes of K) 0.345 us at 256 columns, 0.20 at 128, 0.16 at 64
+//     (the loads of A then bind), a round at least the epilogue of a tile, plus the start and the last tile's epilogue.
 //   cols_kernel: rounds of clusters, each CTA 4 us (start, join) plus its stages; a stage takes its share of the weights'
 //     stream from memory, or the tensor cores' and L2's time for its tokens.
 struct PairPlan
@@ -905,7 +923,8 @@ inline PairPlan pair_plan(int nprob, const Epi* e, bool gated, bool narrow_ok, i
         const int width = gated ? BN / 2 : BN;
         for (int i = 0; i < nprob; ++i) tiles += (long long) ((e[i].M + 255) / 256) * ((e[i].N + width - 1) / width);
         const double rounds = (double) ((tiles + sms / 2 - 1) / (sms / 2));
-        const double us = 4.0 + rounds * (1.5 + nk * (BN == 256 ? 0.46 : BN == 128 ? 0.29 : 0.21));
+        const double main = nk * (BN == 256 ? 0.345 : BN == 128 ? 0.20 : 0.16), drain = BN == 256 ? 2.4 : BN == 128 ? 1.3 : 0.8;
+        const double us = (BN == 256 ? 6.6 : BN == 128 ? 5.2 : 4.4) + rounds * (main > drain ? main : drain);
         if (us < best.us - 1e-9) best = { BN, us };
     }
     return best;

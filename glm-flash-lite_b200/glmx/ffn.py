@@ -32,16 +32,16 @@ def _on(index: int, stream):
     return None
 
 
-def _rows(t: torch.Tensor, align: int) -> torch.Tensor:
+def _rows(t: torch.Tensor, align: int, pitch_of_copy: int = 64) -> torch.Tensor:
     """t [R, n] as rows of packed elements whose distance is a multiple of `align` elements and whose start is 16-byte
-    aligned; copied where it is not."""
+    aligned; where it is not, a copy with rows a multiple of pitch_of_copy elements apart."""
     pitch, inner = t.stride()
     if inner == 1 and pitch % align == 0 and pitch >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     R, n = t.shape
     if R == 1 and inner == 1 and n % align == 0 and t.data_ptr() % 16 == 0:
         return t.as_strided((1, n), (n, 1))
-    c = torch.empty((R, (n + align - 1) // align * align), dtype=t.dtype, device=t.device)[:, :n]
+    c = torch.empty((R, (n + pitch_of_copy - 1) // pitch_of_copy * pitch_of_copy), dtype=t.dtype, device=t.device)[:, :n]
     c.copy_(t)
     return c
 
@@ -68,6 +68,7 @@ class GatedFFN:
         if not act_limit >= 0.0:
             raise ValueError("act_limit must be 0 (none) or positive")
         self._index = w_gate.get_device()
+        self._pitch = (self.I + 63) // 64 * 64           # GLMX_FFN_PITCH: elements between hidden rows
         with torch.cuda.device(self._index):
             pack = lambda w: w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
             self.w_gate, self.w_up, self.w_down = (pack(w.detach()) for w in (w_gate, w_up, w_down))
@@ -117,7 +118,7 @@ class GatedFFN:
                 raise TypeError(f"out must be {self.dtype} or fp32")
         n = x2.shape[0]
         if n:
-            self._run(x2, out, 1 if accumulate else 0, self._new((n, self.I)), 0, 0)
+            self._run(x2, out, 1 if accumulate else 0, self._new((n, self._pitch)), 0, 0)
         return out
 
     __call__ = forward
@@ -132,7 +133,7 @@ class GatedFFN:
                 return self.forward_train(x)
         x2 = self._in(x, "x")
         n = x2.shape[0]
-        y, h, pq = self._new(x.shape), self._new((n, self.I)), self._new((2, n, self.I), torch.float32)
+        y, h, pq = self._new(x.shape), self._new((n, self._pitch)), self._new((2, n, self.I), torch.float32)
         if n:
             p = pq.data_ptr()
             self._run(x2, y, 0, h, p, p + 4 * n * self.I)
@@ -154,11 +155,11 @@ class GatedFFN:
         dwg = new((I, H)) if need[1] else None
         dwu = new((I, H)) if need[2] else None
         dwd = new((H, I)) if need[3] else None
-        inner = new((2, n, I)) if n and (need[0] or need[1] or need[2]) else None
+        inner = new((2, n, self._pitch)) if n and (need[0] or need[1] or need[2]) else None
         ptr = lambda t: 0 if t is None else t.data_ptr()
         p, g = pq.data_ptr(), ptr(inner)
         rc = self.lib.glmx_ffn_backward(self._ref, dy2.data_ptr(), dy2.stride(0) if n else H, x.data_ptr(), x.stride(0) if n else H, n,
-                                        h.data_ptr(), p, p + 4 * n * I, g, g and g + 2 * n * I, ptr(dx), ptr(dwg), ptr(dwu),
+                                        h.data_ptr(), p, p + 4 * n * I, g, g and g + 2 * n * self._pitch, ptr(dx), ptr(dwg), ptr(dwu),
                                         ptr(dwd), _raw_stream(self._index))
         if rc:
             check(rc)

@@ -14,13 +14,15 @@ from ._lib import check
 from .ffn import _on, _raw_stream, _rows
 from .layer import _dt
 
+_PITCH = 128      # bytes between rows that are laid out here: whole lines (the product takes any multiple of 16)
 _FLOAT = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def quantize_rows(x: torch.Tensor, stream=None):
     """x [..., K] fp16 / bf16 / fp32 -> (q int8 [..., K], scale fp32 [...]): scale = max |row| / 127, q = row / scale
     rounded to the nearest integer, ties to even (zeros and scale 0 for a row of zeros; a NaN in a row makes its scale
-    NaN). Rows of q are 16-byte aligned: the last dimension is a slice of a wider buffer where K is not a multiple of 16."""
+    NaN). Rows of q are 128 bytes aligned: the last dimension is a slice of a wider buffer where K is not a multiple
+    of 128."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must be [..., K] with K >= 1")
     if x.dtype not in _FLOAT:
@@ -40,7 +42,7 @@ def quantize_rows(x: torch.Tensor, stream=None):
         x2 = x2.contiguous()
         pitch = K
     R = x2.shape[0]
-    qp = (K + 15) // 16 * 16
+    qp = (K + _PITCH - 1) // _PITCH * _PITCH
     q = torch.empty((R, qp), dtype=torch.int8, device=x.device)
     s = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
     rc = _lib.load().glmx_quantize_rows(x2.data_ptr(), _dt(x2), pitch, R, K, q.data_ptr(), qp, s.data_ptr(), _raw_stream(index))
@@ -56,7 +58,7 @@ def _q_rows(t: torch.Tensor, what: str, K: int) -> torch.Tensor:
         raise ValueError(f"{what} must be int8 [..., {K}]")
     if t.dim() != 2:
         t = t.as_strided((t.numel() // K, K), (t.stride(-2), 1), t.storage_offset()) if _collapses(t) else t.reshape(-1, K)
-    return _rows(t, 16)
+    return _rows(t, 16, _PITCH)
 
 
 def _collapses(t: torch.Tensor) -> bool:
@@ -90,7 +92,7 @@ class Int8Linear:
         self.device, self.out_dtype = wq.device, out_dtype
         self._index = wq.get_device()
         with torch.cuda.device(self._index):
-            self.wq = _rows(wq, 16)
+            self.wq = _rows(wq, 16, _PITCH)
             self.w_scale = _vec(w_scale, self.N, "w_scale", self.device)
             self.bias = None if bias is None else _vec(bias, self.N, "bias", self.device)
         self._w, self._ldw, self._ws = self.wq.data_ptr(), self.wq.stride(0), self.w_scale.data_ptr()

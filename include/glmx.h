@@ -299,16 +299,17 @@ typedef struct
 } glmx_ffn;
 
 /* y [ntok][H] (y_dtype: the block's dtype or GLMX_F32; accumulate = 1 adds to what y holds) from x [ntok] rows of H, ldx
- * elements apart (a multiple of 8, at least H), y rows ldy apart (at least H). h: caller's scratch [ntok][I], 16-byte aligned; it holds the hidden
- * rows afterwards. p, q: fp32 [ntok][I] or both NULL; with them the two factors of the backward pass are kept,
+ * elements apart (a multiple of 8, at least H), y rows ldy apart (at least H). h: caller's scratch, ntok rows of
+ * GLMX_FFN_PITCH(I) elements, 16-byte aligned; it holds the hidden rows afterwards. p, q: fp32 [ntok][I] or both NULL; with them the two factors of the backward pass are kept,
  *   p = min(silu(g), L) * [|u| <= L],  q = clamp(u, -L, L) * silu'(g) * [silu(g) <= L]
  * so that du = dh * p and dg = dh * q. */
+#define GLMX_FFN_PITCH(I) (((I) + 63) / 64 * 64)
 GLMX_API int glmx_ffn_forward(const glmx_ffn* ffn, const void* x, long long ldx, int ntok, void* y, long long ldy,
                               int y_dtype, int accumulate, void* h, float* p, float* q, void* stream);
 
 /* Gradients of glmx_ffn_forward (accumulate = 0) for dy [ntok][H] (rows lddy apart), from the x, h, p and q of the forward call: dx
  * [ntok][H], dw_gate / dw_up [I][H], dw_down [H][I], all in the block's dtype, rows packed; a NULL one is not computed.
- * dg, du: caller's scratch [ntok][I] each in the block's dtype (the gradients of g and u afterwards), 16-byte aligned; not needed (NULL) where only
+ * dg, du: caller's scratch like h, one each (the gradients of g and u afterwards); not needed (NULL) where only
  * dw_down is asked for. */
 GLMX_API int glmx_ffn_backward(const glmx_ffn* ffn, const void* dy, long long lddy, const void* x, long long ldx, int ntok,
                                const void* h, const float* p, const float* q, void* dg, void* du, void* dx, void* dw_gate,
