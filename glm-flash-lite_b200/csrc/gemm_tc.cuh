@@ -538,92 +538,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             tc_after();
             const Epi e = a.e[p];       // in registers: the stores in between would have it read again
             const uint32_t tq = tmem + ((uint32_t) (32 * q) << 16) + (uint32_t) (acc * 256);
-            // this warp's half of the tile's columns, 32 at a time (GATED: 16 of gate and of up): a lane holds a row, and through shared memory
-            // each 8 (4) lanes get 4 columns each of one row, so that global accesses run along rows
-            const int cols = EPI == EPI_GATED ? BN / 4 : BN / 2, c0 = half * cols;
-            constexpr int CC = EPI == EPI_GATED ? 16 : 32, LPR = CC / 4;
-            if (EPI == EPI_I8 || (EPI == EPI_STORE && !e.accumulate))
-                {
-                    // whole rows of 128 bytes (64 or 32 columns) into the staging tile, from there by TMA, or row by row where the
-                    // output's rows are not 16-byte aligned
-                    const int row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
-                    const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
-                    const float xs = EPI == EPI_I8 && row0 + lane < e.M ? e.xs[row0 + lane] : 0.0f;
-                    const int wide = f32 ? 32 : 64, share = max(wide, BN / 2);   // (of a narrow tile, one warp takes all columns)
-                    for (int c = half * share; c < min(BN, (half + 1) * share); c += wide)
-                    {
-                        const int n0 = n * BN + c;
-                        if (lane == 0) tma_store_read();                   // the tile before has been read
-                        __syncwarp();
-                        for (int d = 0; d < wide; d += 16)
-                        {
-                            uint32_t v[16];
-                            tc_ld16(tq + (uint32_t) (c + d), v);
-                            tc_wait_ld();
-                            if constexpr (EPI == EPI_I8)
-                            {
-#pragma unroll
-                                for (int i = 0; i < 16; ++i)
-                                {
-                                    const int col = min(n0 + d + i, e.N - 1);
-                                    float f = (float) (int) v[i] * (xs * __ldg(e.ws + col));
-                                    if (e.bias) f += __ldg(e.bias + col);
-                                    v[i] = __float_as_uint(f);
-                                }
-                            }
-                            if (f32)
-                            {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) stg[lane * 8 + ((d / 4 + i) ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                            }
-                            else
-                            {
-                                uint32_t w[8];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) w[i] = pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), bf);
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) stg[lane * 8 + ((d / 8 + i) ^ (lane & 7))] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                            }
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (!e.vec)
-                        {
-                            copy_rows(e, stg, row0, n0, wide, lane);
-                            __syncwarp();
-                        }
-                        else if (lane == 0 && row0 < e.M && n0 < e.N) tma_store_2d(&maps.y[p], n0, row0, smem_u32(stg));
-                    }
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_remote(map_rank(smem_u32(&tempty[acc]), 0));
-                    continue;
-                }
-            for (int c = c0; c < c0 + cols; c += CC)
+            const bool staged = EPI == EPI_I8 || (EPI == EPI_STORE && !e.accumulate);
+            if (staged)
             {
-                uint32_t v[16], u[16];
-                tc_ld16(tq + (uint32_t) c, v);
-                tc_ld16(tq + (uint32_t) (EPI == EPI_GATED ? BN / 2 + c : c + 16), u);
-                tc_wait_ld();
-                // 16-byte piece i of row r sits at place i ^ (r & 7)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+                // whole rows of 128 bytes (64 or 32 columns) into the staging tile, from there by TMA, or row by row where the
+                // output's rows are not 16-byte aligned
+                const int row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
+                const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
+                const float xs = EPI == EPI_I8 && row0 + lane < e.M ? e.xs[row0 + lane] : 0.0f;
+                const int wide = f32 ? 32 : 64, share = max(wide, BN / 2);   // (of a narrow tile, one warp takes all columns)
+                for (int c = half * share; c < min(BN, (half + 1) * share); c += wide)
                 {
-                    stg[lane * 8 + (i ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    stg[lane * 8 + ((i + 4) ^ (lane & 7))] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-                }
-                __syncwarp();
-                const int nn = n * (EPI == EPI_GATED ? BN / 2 : BN) + c, row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
+                    const int n0 = n * BN + c;
+                    if (lane == 0) tma_store_read();                   // the tile before has been read
+                    __syncwarp();
+                    for (int d = 0; d < wide; d += 16)
+                    {
+                        uint32_t v[16];
+                        tc_ld16(tq + (uint32_t) (c + d), v);
+                        tc_wait_ld();
+                        if constexpr (EPI == EPI_I8)
+                        {
 #pragma unroll
-                for (int i = 0; i < LPR; ++i)
-                {
-                    const int r = i * (32 / LPR) + lane / LPR, pc = lane % LPR;
-                    const uint4 x = stg[r * 8 + (pc ^ (r & 7))], y = EPI == EPI_GATED ? stg[r * 8 + ((pc + 4) ^ (r & 7))] : x;
-                    const uint32_t x4[4] = { x.x, x.y, x.z, x.w }, y4[4] = { y.x, y.y, y.z, y.w };
-                    emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4, y4);
+                            for (int i = 0; i < 16; ++i)
+                            {
+                                const int col = min(n0 + d + i, e.N - 1);
+                                float f = (float) (int) v[i] * (xs * __ldg(e.ws + col));
+                                if (e.bias) f += __ldg(e.bias + col);
+                                v[i] = __float_as_uint(f);
+                            }
+                        }
+                        if (f32)
+                        {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) stg[lane * 8 + ((d / 4 + i) ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        }
+                        else
+                        {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) w[i] = pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), bf);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) stg[lane * 8 + ((d / 8 + i) ^ (lane & 7))] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (!e.vec)
+                    {
+                        copy_rows(e, stg, row0, n0, wide, lane);
+                        __syncwarp();
+                    }
+                    else if (lane == 0 && row0 < e.M && n0 < e.N) tma_store_2d(&maps.y[p], n0, row0, smem_u32(stg));
                 }
-                __syncwarp();
             }
+            if constexpr (EPI != EPI_I8)
+                if (!staged)
+                {
+                    // this warp's half of the tile's columns, 32 at a time (GATED: 16 of gate and of up): a lane holds a row, and through shared memory
+                    // each 8 (4) lanes get 4 columns each of one row, so that global accesses run along rows
+                    const int cols = EPI == EPI_GATED ? BN / 4 : BN / 2, c0 = half * cols;
+                    constexpr int CC = EPI == EPI_GATED ? 16 : 32, LPR = CC / 4;
+                    for (int c = c0; c < c0 + cols; c += CC)
+                    {
+                        uint32_t v[16], u[16];
+                        tc_ld16(tq + (uint32_t) c, v);
+                        tc_ld16(tq + (uint32_t) (EPI == EPI_GATED ? BN / 2 + c : c + 16), u);
+                        tc_wait_ld();
+                        // 16-byte piece i of row r sits at place i ^ (r & 7)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                        {
+                            stg[lane * 8 + (i ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                            stg[lane * 8 + ((i + 4) ^ (lane & 7))] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                        }
+                        __syncwarp();
+                        const int nn = n * (EPI == EPI_GATED ? BN / 2 : BN) + c, row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
+#pragma unroll
+                        for (int i = 0; i < LPR; ++i)
+                        {
+                            const int r = i * (32 / LPR) + lane / LPR, pc = lane % LPR;
+                            const uint4 x = stg[r * 8 + (pc ^ (r & 7))], y = EPI == EPI_GATED ? stg[r * 8 + ((pc + 4) ^ (r & 7))] : x;
+                            const uint32_t x4[4] = { x.x, x.y, x.z, x.w }, y4[4] = { y.x, y.y, y.z, y.w };
+                            emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4, y4);
+                        }
+                        __syncwarp();
+                    }
+                }
             tc_before();
             __syncwarp();
             if (lane == 0) arrive_remote(map_rank(smem_u32(&tempty[acc]), 0));
@@ -655,6 +656,8 @@ struct ColsArgs
 {
     int nseg, K, bk;
     int NT;                     // tokens per tile: a multiple of 16, at most 256
+    int xrows;                  // rows of a token box: NT, or all tokens where there are fewer (the MMA's other columns are not read, and
+                                // rows outside of the matrix would cost the copy more than others do)
     int stages;
     int mtiles;                 // weight-row tiles; the grid is [splits][mtiles * token tiles]
     int tcols;                  // tensor-memory columns: a power of 2 >= NT, at least 32
@@ -682,6 +685,7 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
     const int ksteps = (a.K + a.bk - 1) / a.bk, nk_all = ksteps * a.nseg;
     const int k0 = (int) ((long long) nk_all * split / splits), nk = (int) ((long long) nk_all * (split + 1) / splits) - k0;
     const int rows = EPI == EPI_GATED ? 64 : 128;          // output columns (weight rows of one matrix) per tile
+    const uint32_t tx = 16384u + (uint32_t) a.xrows * 128;
     // next stage to load: segment and place in it
     int seg = k0 / ksteps, kc = (k0 - seg * ksteps) * a.bk;
     const int kend = ksteps * a.bk;
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
     };
     auto load_w = [&](int s, int sg, int c) {
         uint8_t* sw = smem + (size_t) s * STAGE;
-        mbar_arrive_expect_tx(&full[s], (uint32_t) STAGE);
+        mbar_arrive_expect_tx(&full[s], tx);
         if constexpr (EPI == EPI_GATED)
             for (int j = 0; j < 2; ++j) tma_load_2d(sw + j * 8192, &maps.w[j], c, mtile * 64, &full[s]);
         else if constexpr (W_MN)
@@ -903,11 +907,15 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
     return launch_chained(kernel, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), (size_t) pair_smem(BN), st, maps, a);
 }
 
-// Seconds of a launch, in microseconds, by a simple model of what was measured on a B200; the kernel and its tiling are those of the least.
+// Microseconds of a launch by a simple model of what was measured on a B200; the kernel and its tiling are those of the least.
 //   pair_kernel: rounds of tiles over the pairs, each stage (128 bytes of K) 0.345 us at 256 columns, 0.20 at 128, 0.16 at 64
-//     (the loads of A then bind), a round at least the epilogue of a tile, plus the start and the last tile's epilogue.
-//   cols_kernel: rounds of clusters, each CTA 4 us (start, join) plus its stages; a stage takes its share of the weights'
-//     stream from memory, or the tensor cores' and L2's time for its tokens.
+//     (the loads of A then bind) or its share of the weights' stream from memory, a round at least the epilogue of a tile, plus the
+//     start and the last tile's epilogue.
+//   cols_kernel: rounds of clusters, each CTA 3.4 us and 0.018 per token column (start, join) plus its stages on the tensor
+//     cores; or the stream of all tiles' weights from memory (5.9 TB/s), or of all stages from L2 (9 TB/s).
+// E.g. (measured, us, cols / pair 64 / 128 / 256): feed-forward at H = 6144, I = 1536 of 1 row 18 / 54 / 38 / 45, of 200 rows 29 / 33
+// / 31 / 48, of 512 48 / 53 / 37 / 49, of 4096 263 / 272 / 184 / 163; int8 1024 x 1024 of 48 rows 4.6 / 5.8 / 6.4 / 8.8, of 512 9.5
+// / 5.8 / 6.7 / 9.3.
 struct PairPlan
 {
     int BN;
@@ -923,7 +931,10 @@ inline PairPlan pair_plan(int nprob, const Epi* e, bool gated, bool narrow_ok, i
         const int width = gated ? BN / 2 : BN;
         for (int i = 0; i < nprob; ++i) tiles += (long long) ((e[i].M + 255) / 256) * ((e[i].N + width - 1) / width);
         const double rounds = (double) ((tiles + sms / 2 - 1) / (sms / 2));
-        const double main = nk * (BN == 256 ? 0.345 : BN == 128 ? 0.20 : 0.16), drain = BN == 256 ? 2.4 : BN == 128 ? 1.3 : 0.8;
+        double step = BN == 256 ? 0.345 : BN == 128 ? 0.20 : 0.16;
+        const double active = (double) (tiles < sms / 2 ? tiles : sms / 2), stream = active * BN * 128 / ((e[0].M + 255) / 256) / 5.4e6;
+        if (nprob == 1 && stream > step) step = stream;
+        const double main = nk * step, drain = BN == 256 ? 2.6 : BN == 128 ? 2.0 : 1.2;
         const double us = (BN == 256 ? 6.6 : BN == 128 ? 5.2 : 4.4) + rounds * (main > drain ? main : drain);
         if (us < best.us - 1e-9) best = { BN, us };
     }
@@ -960,11 +971,10 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms, const ColsC
     {
         const int room = cap.n[one][s];
         if (room < 1) continue;
-        const long long rounds = (tiles + room - 1) / room;
-        const double ctas = (double) (tiles < room ? tiles : room) * s;              // running at once
-        const double stream = ctas * 16384 / 5.5e6, l2 = ctas * stage / 9.0e6, mma = 0.2 + p.NT * 0.0016;
-        const double step = (stream > l2 ? stream : l2) > mma ? (stream > l2 ? stream : l2) : mma;
-        const double us = rounds * (4.0 + (double) ((nk + s - 1) / s) * step);
+        const double rounds = (double) ((tiles + room - 1) / room), own = 3.4 + 0.018 * p.NT;
+        const double tc = rounds * (own + (double) ((nk + s - 1) / s) * (0.2 + 0.0016 * p.NT));
+        const double hbm = own + (double) p.mtiles * nk * 16384 / 5.9e6, l2 = own + (double) tiles * nk * stage / 9.0e6;
+        const double most = tc > hbm ? tc : hbm, us = (most > l2 ? most : l2) + 0.05 * s;
         if (us < p.us - 1e-9) { p.us = us; p.splits = s; }
     }
     (void) sms;
@@ -1015,7 +1025,7 @@ cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, const Col
     ColsMaps maps;
     ColsArgs a{};
     a.nseg = nseg; a.K = K; a.bk = I8 ? 128 : 64;
-    a.NT = p.NT; a.stages = p.stages; a.mtiles = p.mtiles; a.prefetch = prefetch;
+    a.NT = p.NT; a.xrows = pr.e.M < p.NT ? pr.e.M : p.NT; a.stages = p.stages; a.mtiles = p.mtiles; a.prefetch = prefetch;
     a.tcols = 32;
     while (a.tcols < p.NT) a.tcols *= 2;
     a.idesc = tc_idesc(I8, dtype == GLMX_BF16, W_MN, false, 128, p.NT);
@@ -1024,7 +1034,7 @@ cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, const Col
     for (int i = 0; i < (EPI == EPI_GATED ? 2 : nseg); ++i)
         if ((err = dense_map(&maps.w[i], dtype, pr.b[i], W_MN ? 64 : a.bk, W_MN || EPI == EPI_GATED ? 64 : 128)) != cudaSuccess) return err;
     for (int i = 0; i < nseg; ++i)
-        if ((err = dense_map(&maps.x[i], dtype, pr.a[i], a.bk, p.NT)) != cudaSuccess) return err;
+        if ((err = dense_map(&maps.x[i], dtype, pr.a[i], a.bk, a.xrows)) != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.mtiles * p.ttiles);
     cfg.blockDim = dim3(COLS_THREADS);
