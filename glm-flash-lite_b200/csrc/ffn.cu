@@ -62,7 +62,7 @@ extern "C" int glmx_ffn_forward(const glmx_ffn* f, const void* x, long long ldx,
     g.b[0] = { f->w_gate, I, H, H };
     g.b[1] = { f->w_up, I, H, H };
     g.e = epi(f, ntok, I);
-    g.e.o0 = h; g.e.ldo = P; g.e.p = p; g.e.q = q;
+    g.e.o0 = h; g.e.ldo = P; g.e.p = p; g.e.q = q; g.e.x = x; g.e.wg = f->w_gate; g.e.wu = f->w_up; g.e.ldx = ldx; g.e.K = H;
     cudaError_t e = launch_product<false, false, EPI_GATED>(f->dtype, g, 1, H, false, st);
     if (e == cudaSuccess)
     {

@@ -30,6 +30,7 @@ struct Epi
     long long ldo;
     float* p; float* q;         // [M][N]
     float limit;
+    const void* x; const void* wg; const void* wu; long long ldx; int K;   // GATED with p: the operands, for the sums next to the limit
     const float* xs; const float* ws; const float* bias; // I8
 };
 
@@ -66,36 +67,99 @@ __device__ __forceinline__ void store_f32(float* d, const float (&v)[W])
     for (int i = 0; i < W / 4; ++i) reinterpret_cast<float4*>(d)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
 
-// W (4, or 1 where rows cannot take wide stores) consecutive columns n .. n + W - 1 of token t; n is a multiple of W. acc: the sums (GATED: of
-// gate; acc2 of up). I8 sums are int32 bit patterns.
+// sum_k x[t][k] w[n][k] in 64 bits by a warp (K a multiple of 8, both rows 16-byte aligned)
+static __device__ __noinline__ double warp_dot(const void* x, const void* w, int K, int bf16)
+{
+    double d = 0.0;
+    for (int k = (threadIdx.x & 31) * 8; k < K; k += 256)
+    {
+        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + k);
+        const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d += (double) load16(&a, i, bf16) * (double) load16(&b, i, bf16);
+    }
+    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    return d;
+}
+
+// h (and p, q) of 4 consecutive columns n .. n + 3 of token t, a multiple of 4; called by whole warps. acc, acc2: the sums of gate and up.
+// Which side of the limit a value falls on decides whether its gradient passes, and so must not hang on the last bits of
+// the tensor cores' truncated sums: within K 2^-25 (half a truncation for each MMA of 16 inputs, 16 times) the sum is formed again in 64 bits.
+__device__ __forceinline__ void emit_gated(const Epi& e, int t, int n, const uint32_t (&acc)[4], const uint32_t (&acc2)[4])
+{
+    // N is a multiple of 8: all columns are inside, or none
+    const bool in = t < e.M && n < e.N;
+    const float L = e.limit;
+    float g[4], u[4], s[4], act[4];
+    bool kg[4], ku[4];
+    uint32_t near = 0;
+    const float win = L * ((float) e.K * 0x1p-25f + 0x1p-18f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        g[i] = __uint_as_float(acc[i]);
+        u[i] = __uint_as_float(acc2[i]);
+        s[i] = __fdividef(1.0f, 1.0f + __expf(-g[i]));
+        act[i] = g[i] < -100.0f ? 0.0f : g[i] * s[i];      // silu(-inf) = 0 (not -inf * 0)
+        kg[i] = L == 0.0f || act[i] <= L;
+        ku[i] = L == 0.0f || fabsf(u[i]) <= L;
+        if (L != 0.0f) near |= (fabsf(act[i] - L) <= win ? 1u : 0u) << i | (fabsf(fabsf(u[i]) - L) <= win ? 16u : 0u) << i;
+    }
+    if (e.p && L != 0.0f)
+    {
+        if (!in) near = 0;
+        uint32_t lanes = __ballot_sync(0xffffffffu, near != 0);
+        while (lanes)
+        {
+            const int src = __ffs(lanes) - 1;
+            lanes &= lanes - 1;
+            uint32_t bits = __shfl_sync(0xffffffffu, near, src);
+            const int tt = __shfl_sync(0xffffffffu, t, src), nn = __shfl_sync(0xffffffffu, n, src);
+            while (bits)
+            {
+                const int b = __ffs(bits) - 1, c = nn + (b & 3);
+                bits &= bits - 1;
+                const double d = warp_dot(static_cast<const uint16_t*>(e.x) + (size_t) tt * e.ldx,
+                                          static_cast<const uint16_t*>(b < 4 ? e.wg : e.wu) + (size_t) c * e.K, e.K, e.bf16);
+                const bool keep = b < 4 ? d / (1.0 + exp(-d)) <= (double) L : fabs(d) <= (double) L;
+                if ((threadIdx.x & 31) == src)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        if (b == i) kg[i] = keep;
+                        if (b == i + 4) ku[i] = keep;
+                    }
+            }
+        }
+    }
+    if (!in) return;
+    float hh[4], pp[4], qq[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        float ac = act[i], up = u[i];
+        if (L != 0.0f)
+        {
+            ac = fminf(ac, L);
+            up = fminf(fmaxf(up, -L), L);
+            if (u[i] != u[i]) up = u[i];                   // NaN stays NaN
+            if (g[i] != g[i]) ac = g[i];
+        }
+        hh[i] = ac * up;
+        pp[i] = ku[i] ? ac : 0.0f;
+        qq[i] = kg[i] ? up * (s[i] + act[i] * (1.0f - s[i])) : 0.0f;
+    }
+    store16<4>(e.o0, (size_t) t * e.ldo + n, hh, e.bf16);
+    const size_t o = (size_t) t * e.N + n;
+    if (e.p) { store_f32<4>(e.p + o, pp); store_f32<4>(e.q + o, qq); }
+}
+
+// W (4, or 1 where rows cannot take wide stores) consecutive columns n .. n + W - 1 of token t; n is a multiple of W. acc: the sums (I8: int32).
 template <int EPI, int W>
-__device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t (&acc)[W], const uint32_t (&acc2)[W])
+__device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t (&acc)[W])
 {
     if (t >= e.M || n >= e.N) return;
     float v[W];
-    if constexpr (EPI == EPI_GATED && W == 4)
-    {
-        // N is a multiple of 8: all W columns are inside
-        const size_t o = (size_t) t * e.N + n;
-        const float L = e.limit;
-        float hh[W], pp[W], qq[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-        {
-            const float g = __uint_as_float(acc[i]), u = __uint_as_float(acc2[i]);
-            const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-            // silu(-inf) = 0 (not -inf * 0)
-            float act = g < -100.0f ? 0.0f : g * s, up = u;
-            const bool kg = L == 0.0f || act <= L, ku = L == 0.0f || fabsf(u) <= L;
-            if (L != 0.0f) { act = fminf(act, L); up = fminf(fmaxf(u, -L), L); if (u != u) up = u; if (g != g) act = g; }
-            hh[i] = act * up;
-            pp[i] = ku ? act : 0.0f;
-            qq[i] = kg ? up * (s + (g < -100.0f ? 0.0f : g * s * (1.0f - s))) : 0.0f;
-        }
-        store16<W>(e.o0, (size_t) t * e.ldo + n, hh, e.bf16);
-        if (e.p) { store_f32<W>(e.p + o, pp); store_f32<W>(e.q + o, qq); }
-        return;
-    }
     if constexpr (EPI == EPI_DACT && W == 4)
     {
         const size_t o = (size_t) t * e.N + n;
@@ -620,7 +684,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                             const int r = i * (32 / LPR) + lane / LPR, pc = lane % LPR;
                             const uint4 x = stg[r * 8 + (pc ^ (r & 7))], y = EPI == EPI_GATED ? stg[r * 8 + ((pc + 4) ^ (r & 7))] : x;
                             const uint32_t x4[4] = { x.x, x.y, x.z, x.w }, y4[4] = { y.x, y.y, y.z, y.w };
-                            emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4, y4);
+                            if constexpr (EPI == EPI_GATED) emit_gated(e, row0 + r, nn + 4 * pc, x4, y4);
+                            else emit<EPI, 4>(e, row0 + r, nn + 4 * pc, x4);
                         }
                         __syncwarp();
                     }
@@ -800,10 +865,13 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
         constexpr int W = decltype(wide)::value;
         const int per = rows / W, units = ncols * per;
         const int u0 = (int) ((long long) units * split / splits), u1 = (int) ((long long) units * (split + 1) / splits);
-        for (int u = u0 + tid; u < u1; u += COLS_THREADS)
+        for (int ub = u0; ub < u1; ub += COLS_THREADS)
         {
+            // (whole warps stay together: the last ones' lanes past the end work on the last unit and drop it)
+            const int u = min(ub + tid, u1 - 1);
+            const bool mine = ub + tid < u1;
             const int c = u / per, r = (u - c * per) * W;
-            uint32_t v[W], w[W];
+            uint32_t v[W];
             auto sum = [&](uint32_t (&d)[W], uint32_t off) {
                 uint32_t x[8][W];
 #pragma unroll
@@ -823,17 +891,25 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
                         for (int i = 0; i < W; ++i) d[i] = I8 ? d[i] + x[rk][i] : __float_as_uint(__fadd_rn(__uint_as_float(d[i]), __uint_as_float(x[rk][i])));
             };
             sum(v, (uint32_t) (c * 128 + r) * 4);
-            if constexpr (EPI == EPI_GATED) sum(w, (uint32_t) (c * 128 + 64 + r) * 4);
+            const int t = mine ? ttile * NT + c : a.e.M;
+            if constexpr (EPI == EPI_GATED)
+            {
+                uint32_t w[W];
+                sum(w, (uint32_t) (c * 128 + 64 + r) * 4);
+                emit_gated(a.e, t, mtile * rows + r, v, w);
+            }
             else
-#pragma unroll
-                for (int i = 0; i < W; ++i) w[i] = v[i];
-            emit<EPI, W>(a.e, ttile * NT + c, mtile * rows + r, v, w);
+                emit<EPI, W>(a.e, t, mtile * rows + r, v);
         }
     };
     if (!s_abort)
     {
-        if (EPI == EPI_I8 && !a.e.vec) join(Int<1>());
-        else join(Int<4>());
+        if constexpr (EPI == EPI_I8)
+        {
+            if (a.e.vec) join(Int<4>()); else join(Int<1>());
+        }
+        else
+            join(Int<4>());
     }
     __syncwarp();
     if (splits > 1) cluster_sync();                        // nobody leaves while its partial tile is read

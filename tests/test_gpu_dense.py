@@ -162,6 +162,25 @@ def test_ffn_backward(dev, T, H, I, dt):
             assert float((a.double() - ref).abs().max()) <= 40 * r(dt) * float(ref.abs().max()) + 64 * tiny(dt), (name, L)
 
 
+@pytest.mark.parametrize("T,H,I", [(5, 6144, 256), (40, 1160, 488), (700, 1032, 776), (1100, 2048, 512)])
+def test_ffn_limit_next_to_values(dev, T, H, I):
+    """Which gradients pass the clamp is decided as in 64 bits, also where the limit is the fp32 number next to a value."""
+    from glmx import GatedFFN
+    x, wg, wu, wd, _ = block(dev, T, H, I, BF, 500 + T)
+    g, u, act, _, _ = plain(x, wg, wu, wd, 0.0)
+    vals = torch.cat([act.flatten(), u.abs().flatten()])
+    vals = vals[(vals > 0.5) & (vals < 3)]
+    pick = torch.randint(0, vals.numel(), (12,), generator=torch.Generator(device=dev).manual_seed(T), device=dev)
+    for v in vals[pick].tolist():
+        L = float(torch.tensor(v, dtype=F32))                # above or below the value, by less than a rounding
+        _, (_, _, pq) = GatedFFN(wg, wu, wd, act_limit=L).forward_train(x)
+        p, q = pq[0], pq[1]
+        # the factors are 0 where the value is past the limit, and only there (or where they are 0 or tiny by themselves)
+        assert torch.equal(p != 0, (u.abs() <= L) & (act.float() != 0))
+        past = act > L
+        assert bool((q[past] == 0).all()) and bool((q[~past & (act > 0.1) & (u.abs() > 1e-3)] != 0).all())
+
+
 def test_ffn_backward_against_differences(dev):
     """Directional differences of the block in 64 bits: <gradient, d> = (f(p + e d) - f(p - e d)) / 2e."""
     from glmx import GatedFFN
