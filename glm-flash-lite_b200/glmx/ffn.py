@@ -69,13 +69,19 @@ class GatedFFN:
             raise ValueError("act_limit must be 0 (none) or positive")
         self._index = w_gate.get_device()
         self._pitch = (self.I + 63) // 64 * 64           # GLMX_FFN_PITCH: elements between hidden rows
-        with torch.cuda.device(self._index):
-            pack = lambda w: w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-            self.w_gate, self.w_up, self.w_down = (pack(w.detach()) for w in (w_gate, w_up, w_down))
+        self.w_gate, self.w_up, self.w_down = self._pack(w_gate), self._pack(w_up), self._pack(w_down)
         self.act_limit = float(act_limit)
         self._desc = _lib.Ffn(self.H, self.I, _dt(w_gate), self.w_gate.data_ptr(), self.w_up.data_ptr(),
                               self.w_down.data_ptr(), self.act_limit)
         self._ref = C.byref(self._desc)
+
+    def _pack(self, w: torch.Tensor) -> torch.Tensor:
+        if w.requires_grad:
+            w = w.detach()
+        if w.is_contiguous() and w.data_ptr() % 16 == 0:
+            return w
+        with torch.cuda.device(self._index):
+            return w.clone(memory_format=torch.contiguous_format)
 
     def _in(self, x: torch.Tensor, what: str) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.H:
@@ -87,7 +93,7 @@ class GatedFFN:
         return _rows(x if x.dim() == 2 else x.reshape(-1, self.H), 8)
 
     def _new(self, shape, dtype=None):
-        return torch.empty(shape, dtype=dtype or self.dtype, device=self.device)
+        return self.w_gate.new_empty(shape) if dtype is None else self.w_gate.new_empty(shape, dtype=dtype)
 
     def _run(self, x, y, accumulate, h, p, q):
         rc = self.lib.glmx_ffn_forward(self._ref, x.data_ptr(), x.stride(0), x.shape[0], y.data_ptr(), self.H, _dt(y), accumulate,

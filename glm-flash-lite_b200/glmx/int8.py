@@ -43,8 +43,8 @@ def quantize_rows(x: torch.Tensor, stream=None):
         pitch = K
     R = x2.shape[0]
     qp = (K + _PITCH - 1) // _PITCH * _PITCH
-    q = torch.empty((R, qp), dtype=torch.int8, device=x.device)
-    s = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    q = x.new_empty((R, qp), dtype=torch.int8)
+    s = x.new_empty(shape[:-1], dtype=torch.float32)
     rc = _lib.load().glmx_quantize_rows(x2.data_ptr(), _dt(x2), pitch, R, K, q.data_ptr(), qp, s.data_ptr(), _raw_stream(index))
     if rc:
         check(rc)
@@ -121,7 +121,7 @@ class Int8Linear:
             dt = out_dtype or self.out_dtype or torch.bfloat16
             if dt not in _FLOAT:
                 raise TypeError("out_dtype must be fp16, bf16 or fp32")
-            out = torch.empty((*xq.shape[:-1], self.N), dtype=dt, device=self.device)
+            out = xq.new_empty((*xq.shape[:-1], self.N), dtype=dt)
         elif tuple(out.shape) != (*xq.shape[:-1], self.N) or not out.is_contiguous() or out.device != self.device or \
                 out.dtype not in _FLOAT:
             raise ValueError("out must be contiguous fp16 / bf16 / fp32 [..., N] on the weights' device")

@@ -62,7 +62,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     k, kp, k0 = _param(top_k, torch.int32, B, index, "top_k")
     p, pp, p0 = _param(top_p, torch.float32, B, index, "top_p")
     m, mp, m0 = _param(min_p, torch.float32, B, index, "min_p")
-    ids = torch.empty(B, dtype=out_dtype, device=logits.device)
+    ids = logits.new_empty(B, dtype=out_dtype)
     rc = _lib.load().glmx_sample(logits.data_ptr(), _dt(logits), max(ld, V), B, V, u.data_ptr(), tp, t0, kp, k0, pp, p0, mp, m0,
                                  ids.data_ptr(), _dt(ids), _raw_stream(index))
     if rc:
