@@ -9,11 +9,14 @@
 // Few logits matter as a rule. The largest logit of each thread's share is known from the load: where k of these lie above a bin's
 // edge, the top k logits do. What lies above is gathered (at most 512 logits, else the general way) and sorted in one
 // CTA, which finishes the row; without a top-k the same is done where the gathered weights reach top_p.
-// Otherwise the threshold is found by a histogram of 1024 bins of m - l, narrowed by histograms over the keys
-// (order-preserving integers) of one bin, and the pick by running sums over the row: the CTA, the warp, then the lane in
-// whose run the target falls.
+// Otherwise the threshold is found by a histogram of 1024 bins of m - l (for top-p of the interval of exponents in which it
+// falls, known from the pass that sums the weights), whose bin is gathered and sorted or, where it holds more than 512 logits, narrowed by histograms over
+// keys (order-preserving integers); and the pick by running sums over the row: the CTA, the warp, then the lane in whose
+// run the target falls.
 #include "dense.h"
 #include "glmx_common.cuh"
+
+#include <cstddef>
 
 namespace glmx {
 
@@ -31,7 +34,8 @@ struct SampleArgs
 
 constexpr int ST = 512, SBINS = 1024, SLIST = 512, SRANKS = 8;
 constexpr int SLICE_MAX = GLMX_SAMPLE_MAX_VOCAB / SRANKS;  // 49152 logits: 192 KB
-constexpr float SPAN = 16.0f;                              // the first histogram's bins reach down to exp(-16); the last holds the rest
+constexpr int NPV = 4;                                     // weights are also summed down to these exponents: a histogram then covers one interval
+__device__ constexpr float PV[NPV + 1] = { 4.0f, 6.5f, 9.0f, 12.0f, 30.6f };   // (exp(-30.5) = 2^-44: what lies further down weighs nothing)
 constexpr int TRY = 320;                                   // without a top-k: thread maxima above the gathered logits' edge
 
 // order-preserving key of a logit that is not NaN; TS bits are the same in all values of the type
@@ -71,7 +75,7 @@ struct Weight
     }
 };
 
-struct Hist
+struct alignas(16) Hist                                    // (cleared in 16-byte pieces)
 {
     uint32_t lo[4][SBINS], hi[SBINS], cnt[SBINS];          // masses in two words (or counts in the low one), counts. Four copies of
                                                            // the low word: lanes that hit one bin meet less often
@@ -86,12 +90,13 @@ struct Found                                               // the bin in which a
 
 struct Shared
 {
-    u64 mail[2][3][SRANKS];
-    u64 warp[ST / 32];
+    u64 mail[2][NPV + 1][SRANKS];
+    u64 part[NPV + 1][ST / 32];
+    u64 warp[ST / 32], result;
     uint32_t warp32[ST / 32];
     u64 list[SLIST];                                       // (logit, id) of the gathered logits, in CTA 0
     uint32_t maxima[SBINS];                                // histogram of the threads' maxima
-    union
+    union alignas(16)
     {
         Hist hist;
         struct { u64 sorted[SLIST]; uint32_t order[SLIST]; };
@@ -200,6 +205,8 @@ __device__ __forceinline__ V sort_n(V v, int n, V* s)
     return v;
 }
 
+static_assert(offsetof(Shared, hist) % 16 == 0 && sizeof(Hist) % 16 == 0, "the histogram is cleared in 16-byte pieces");
+
 template <typename T>
 __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ SampleArgs a)
 {
@@ -229,6 +236,35 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         }
         sync();
         return sl;
+    };
+    // the block's sums of up to NPV + 1 values, from every CTA, in the same way
+    auto exchange_sums = [&](auto... values) {
+        constexpr int N = sizeof...(values);
+        u64 v[N] = { (u64) values... };
+        const int sl = slot;
+        slot ^= 1;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (lane == i) sh.part[i][warp] = v[i];
+        __syncthreads();
+        if (tid < N * NC)
+        {
+            const int i = tid / NC;
+            u64 t = 0;
+            for (int w = 0; w < ST / 32; ++w) t += sh.part[i][w];
+            dsmem_st(&sh.mail[sl][i][rank], tid - i * NC, t);
+        }
+        sync();
+        return sl;
+    };
+    auto total_of = [&](int sl, int i) {
+        u64 t = 0;
+        for (int r = 0; r < NC; ++r) t += sh.mail[sl][i][r];
+        return t;
     };
     auto put = [&](int id) {
         if (a.ids64) static_cast<long long*>(a.ids)[b] = id; else static_cast<int*>(a.ids)[b] = id;
@@ -399,6 +435,22 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     };
 
     u64 S = 0;                                             // the weights' sum, where top-p needs it
+    // a logit into CTA 0's list
+    auto push = [&](float l, int j) {
+        const uint32_t at = dsmem_add(&sh.n_list, 0, 1u);
+        if (at < SLIST) dsmem_st(&sh.list[at], 0, (u64) __float_as_uint(l) << 32 | (uint32_t) (g0 + j));
+    };
+    // element tid of the list's n (at most SLIST) by descending logit, then by id; it is in any order: the sort fixes it. Keys are those of
+    // fp32, from which the logit comes back
+    auto sorted_list = [&](int n_list, float& l, uint32_t& id) {
+        const bool in = tid < n_list;
+        const u64 e = in ? sh.list[tid] : 0ull;
+        u64 s = in ? (u64) key_of<float>(__uint_as_float((uint32_t) (e >> 32))) << 32 | (uint32_t) ~(uint32_t) e : 0ull;
+        s = sort_n(s, n_list, sh.sorted);
+        l = of_key<float>((uint32_t) (s >> 32));
+        id = ~(uint32_t) s;
+        return in;
+    };
     if (by_k || by_p)
     {
         // the edge: the bin at which k of the threads' maxima are reached (without a top-k, TRY of them or all)
@@ -416,50 +468,37 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         const uint32_t cs = block_scan(c0 + c1, sh.warp32, all32);
         const uint32_t want = by_k ? (uint32_t) k : min(all32, (uint32_t) TRY);
         const int edge = crossing(c0, c1, cs, want, c0, c1).bin;   // -1: fewer maxima than k
-        // gathered: what lies up to the edge (and a rounding more); with top-p alone, all weights are summed as well
-        u64 sum = 0, listed = 0;
-        int got = 0;
+        // gathered: what lies up to the edge (and a rounding more), straight into CTA 0's list, so that the others are done once their
+        // shares are in; with top-p alone, all weights are summed as well
         const float floor_l = edge >= 0 ? bin_floor(edge, scale) : INF;
-        auto gather = [&](float l, int j) {
-            if (l >= floor_l && l != NONE)
-            {
-                // straight into CTA 0's list, so that the others are done once their shares are in
-                const uint32_t at = dsmem_add(&sh.n_list, 0, 1u);
-                if (at < SLIST) dsmem_st(&sh.list[at], 0, (u64) __float_as_uint(l) << 32 | (uint32_t) (g0 + j));
-                ++got;
-                if (!by_k) listed += weight(l);
-            }
-        };
-        if (!by_k) each([&](float l, int j) { sum += weight(l); gather(l, j); });
-        else if (mine_max >= floor_l) each(gather);
-        got = __reduce_add_sync(0xffffffffu, got);
-        __syncthreads();
-        if (lane == 0) sh.warp32[warp] = got;
-        if (!by_k) { listed = block_sum(listed); sum = block_sum(sum); } else __syncthreads();
-        got = 0;
-#pragma unroll
-        for (int i = 0; i < ST / 32; ++i) got += sh.warp32[i];
-        const int sl = exchange((u64) got, sum, listed);
-        int total = 0;
-        listed = 0;
-        for (int r = 0; r < NC; ++r)
+        int got = 0, total;
+        u64 listed = 0;
+        if (by_k)
         {
-            total += (int) sh.mail[sl][0][r];
-            S += sh.mail[sl][1][r];
-            listed += sh.mail[sl][2][r];
+            if (mine_max >= floor_l)
+                each([&](float l, int j) { if (l >= floor_l && l != NONE) { push(l, j); ++got; } });
+            total = (int) total_of(exchange_sums(got), 0);
+        }
+        else
+        {
+            u64 sum = 0;
+            each([&](float l, int j) {
+                const u64 w = weight(l);
+                sum += w;
+                if (l >= floor_l && l != NONE) { push(l, j); ++got; listed += w; }
+            });
+            const int sl = exchange_sums(got, listed, sum);
+            total = (int) total_of(sl, 0);
+            listed = total_of(sl, 1);
+            S = total_of(sl, 2);
         }
         if (edge >= 0 && total <= SLIST && (by_k || listed >= need_of(S)))
         {
             if (rank == 0)
             {
-                // the list is in any order: the sort fixes it
-                const bool in = tid < total;
-                const u64 e = in ? sh.list[tid] : 0ull;
-                // by key, then by id: descending (key, ~id); with the key of fp32, from which the logit comes back
-                u64 s = in ? (u64) key_of<float>(__uint_as_float((uint32_t) (e >> 32))) << 32 | (uint32_t) ~(uint32_t) e : 0ull;
-                s = sort_n(s, total, sh.sorted);
-                const uint32_t ky = (uint32_t) (s >> 32), id = ~(uint32_t) s;
-                const float l = of_key<float>(ky);
+                float l;
+                uint32_t id;
+                const bool in = sorted_list(total, l, id);
                 u64 w = in && (!by_k || tid < k) ? weight(l) : 0ull, all;
                 u64 upto = block_scan(w, sh.warp, all);
                 if (by_p && tid > 0 && upto - w >= need_of(by_k ? all : S)) w = 0;
@@ -491,7 +530,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         Hist& h = sh.hist;
         sync();                                            // nobody reads an earlier one
         for (int i = tid; i < (int) (sizeof(Hist) / 16); i += ST) reinterpret_cast<uint4*>(&h)[i] = make_uint4(0, 0, 0, 0);
-        if (tid == 0) sh.found.bin = -1;
+        if (tid == 0) { sh.found.bin = -1; sh.n_list = 0; }
         __syncthreads();
         each([&](float l, int j) {
             const int q = l != NONE && kept(l, j) ? bin(l) : -1;
@@ -552,7 +591,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     // sum of f over the slice; `mine` gets this warp's part
     auto slice_sum = [&](auto f, u64& mine) {
         mine = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (int j = j0 + lane * 4; j < j1; j += 128)
         {
             const float4 v = *reinterpret_cast<const float4*>(lg + j);
@@ -592,14 +631,34 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
             }
     };
 
-    // from a bin of m - l (of that scale) to the exact threshold, in thr and cut
-    auto narrow = [&](bool mass, u64 need, Found f, float scale) {
-        const int b0 = f.bin;
+    // from a bin, gathered and sorted in CTA 0, to the exact threshold, in thr and cut; false where it holds too many
+    auto resolve = [&](bool mass, u64 need, const Found& f, auto in_bin) {
+        int got = 0;
+        each([&](float l, int j) { if (in_bin(l, j)) { push(l, j); ++got; } });
+        const int total = (int) total_of(exchange_sums(got), 0);
+        if (total > SLIST) return false;
+        if (rank == 0)
+        {
+            float l;
+            uint32_t id;
+            const bool in = sorted_list(total, l, id);
+            const u64 w = in ? mass ? weight(l) : 1ull : 0ull, rest = need - f.above;
+            u64 all;
+            const u64 upto = block_scan(w, sh.warp, all);
+            if (upto - w < rest && upto >= rest)
+                for (int r = 0; r < NC; ++r) dsmem_st(&sh.result, r, (u64) __float_as_uint(l) << 32 | id);
+        }
+        sync();
+        thr = __uint_as_float((uint32_t) (sh.result >> 32));
+        cut = (int) (uint32_t) sh.result;
+        return true;
+    };
+    // the same by histograms over the keys of the bin's logits
+    auto narrow = [&](bool mass, u64 need, Found f, auto in_bin) {
         u64 above = f.above;
         uint32_t lo = 0xffffffffu, hi = 0, cnt = 0;
-        const float floor_l = bin_floor(b0, scale);
         each([&](float l, int j) {
-            if (!(l >= floor_l) || l == NONE || bin_at(l, scale) != b0 || !kept(l, j)) return;
+            if (!in_bin(l, j)) return;
             const uint32_t ky = key_of<T>(l);
             lo = min(lo, ky);
             hi = max(hi, ky);
@@ -676,20 +735,47 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         for (int r = 0; r < NC; ++r) kl = min(kl, (uint32_t) sh.mail[sl][0][r]);
         const float scale = bin_scale(mx - of_key<float>(kl));
         const Found f = histogram(false, false, (u64) k, [&](float l) { return bin_at(l, scale); });
-        if (f.bin >= 0) narrow(false, (u64) k, f, scale);  // else: fewer than k logits may be picked at all
-        if (by_p)
+        if (f.bin >= 0)                                    // else: fewer than k logits may be picked at all
         {
-            u64 mine, before;
-            const u64 sum = slice_sum([&](float l, int j) { return kept(l, j) ? weight(l) : 0ull; }, mine);
-            spread(sum, before, S);
+            const float floor_l = bin_floor(f.bin, scale);
+            auto in_bin = [&](float l, int) { return l >= floor_l && l != NONE && bin_at(l, scale) == f.bin; };
+            if (!resolve(false, (u64) k, f, in_bin)) narrow(false, (u64) k, f, in_bin);
         }
     }
     if (by_p)
     {
-        const u64 need = need_of(S);
-        const float scale = bin_scale(fminf(SPAN * T0, mx - fmaxf(thr, -3.0e38f)));
-        const Found f = histogram(true, false, need, [&](float l) { return bin_at(l, scale); });
-        narrow(true, need, f, scale);
+        // the kept weights' sum S and M, the sums from each pv up; the interval of exponents in which top_p * S is reached
+        float pv[NPV];
+        u64 M[NPV] = {};
+        S = 0;
+#pragma unroll
+        for (int i = 0; i < NPV; ++i) pv[i] = mx - PV[i] * T0;
+        each([&](float l, int j) {
+            const u64 w = kept(l, j) ? weight(l) : 0ull;
+            S += w;
+#pragma unroll
+            for (int i = 0; i < NPV; ++i) M[i] += l >= pv[i] ? w : 0ull;
+        });
+        const int sl = exchange_sums(S, M[0], M[1], M[2], M[3]);
+        S = total_of(sl, 0);
+#pragma unroll
+        for (int i = 0; i < NPV; ++i) M[i] = total_of(sl, 1 + i);
+        u64 need = need_of(S), above = 0;
+        float top = mx, low = NONE, below = INF, width = PV[NPV] - PV[NPV - 1];
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < NPV; ++i)
+            if (open)
+            {
+                if (M[i] >= need) { low = pv[i]; width = PV[i] - (i ? PV[i - 1] : 0.0f); open = false; }
+                else { above = M[i]; top = below = pv[i]; }
+            }
+        need -= above;
+        const float scale = bin_scale(width * T0);
+        auto bin = [&](float l) { return l >= low && l < below ? (int) fminf((top - l) * scale, 1023.0f) : -1; };
+        const Found f = histogram(true, false, need, bin);
+        auto in_bin = [&](float l, int j) { return l != NONE && bin(l) == f.bin && kept(l, j); };
+        if (!resolve(true, need, f, in_bin)) narrow(true, need, f, in_bin);
     }
     u64 mine, before, all;
     auto pick = [&](auto final_weight) {
