@@ -6,31 +6,108 @@ namespace glmx {
 
 namespace {
 
-// One CTA per row: the row's largest magnitude, then its quotients (the second read comes from cache). Bound by the read
-// of x. Quotients and the scale are IEEE divisions, so that the integers follow from the definition alone.
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* x, long long ldx, int K, signed char* q, long long ldq, float* scale)
+constexpr int QT = 256;
+
+// The block's largest magnitude, of fp32 bit patterns without sign: as integers they are in order, infinity next to last and NaN
+// above it, so that a NaN anywhere is the result and shows in the row's scale and so in every output of the row.
+__device__ __forceinline__ float block_amax(uint32_t m)
 {
-    const T* xr = x + (size_t) blockIdx.x * ldx;
-    float m = 0.0f;
-    bool nan = false;
-    for (int k = threadIdx.x; k < K; k += 256)
-    {
-        const float v = to_f32(xr[k]);
-        nan |= v != v;
-        m = fmaxf(m, fabsf(v));
-    }
-    __shared__ float sm[8];
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    __shared__ uint32_t sm[QT / 32];
+    m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m;
-    nan = __syncthreads_or(nan);
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, sm[w]);
-    // a NaN in the row shows in its scale, and so in every output of the row
-    const float s = nan ? __int_as_float(0x7fc00000) : __fdiv_rn(m, 127.0f);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < QT / 32; ++w) m = max(m, sm[w]);
+    return __uint_as_float(m);
+}
+
+__device__ __forceinline__ int quantise(float x, float s)
+{
+    return s > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(x, s)))) : 0;
+}
+
+// Rows of whole 16-byte groups: a CTA holds its row in registers (NV groups a thread), so that x is read once, and the quotients cost a
+// product each: x / s is within 127 * 1.5 * 2^-23 < 2^-15 of it, so that only a group with a value that near a half has to divide.
+// Adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low byte. Bound by the reads: 4096 rows of 6144 in
+// bf16 21 us (75 MB, 3.6 TB/s; 30 us by the kernel below), one row 3.2 us.
+template <typename T, int NV>
+__global__ void __launch_bounds__(QT) quantize_kernel(const T* x, long long ldx, int K, signed char* q, long long ldq, float* scale)
+{
+    constexpr int G = 16 / sizeof(T);
+    grid_release();
+    const uint4* xr = reinterpret_cast<const uint4*>(x + (size_t) blockIdx.x * ldx);
+    const int ng = K / G;
+    uint4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+    {
+        const int g = threadIdx.x + i * QT;
+        v[i] = g < ng ? __ldcs(xr + g) : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < G; ++j) m = max(m, __float_as_uint(to_f32(reinterpret_cast<const T*>(&v[i])[j])) & 0x7fffffffu);
+    const float s = __fdiv_rn(block_amax(m), 127.0f);
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+    const float inv = 1.0f / s;
+    const bool plain = s > 0x1p-100f && s < 0x1p100f;      // 1 / s is a normal number
+    signed char* qr = q + (size_t) blockIdx.x * ldq;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+    {
+        const int g = threadIdx.x + i * QT;
+        if (g >= ng) break;
+        const T* e = reinterpret_cast<const T*>(&v[i]);
+        uint32_t n[G];
+        float off = 0.0f;
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+        {
+            const float r = to_f32(e[j]) * inv, f = r + 12582912.0f;
+            off = fmaxf(off, fabsf(r - (f - 12582912.0f)));
+            n[j] = __float_as_uint(f);
+        }
+        if (!plain || off > 0.5f - 0x1p-14f)
+#pragma unroll
+            for (int j = 0; j < G; ++j) n[j] = (uint32_t) quantise(to_f32(e[j]), s);
+        uint32_t w[G / 4];
+#pragma unroll
+        for (int j = 0; j < G / 4; ++j)
+            w[j] = __byte_perm(__byte_perm(n[4 * j], n[4 * j + 1], 0x0040), __byte_perm(n[4 * j + 2], n[4 * j + 3], 0x0040), 0x5410);
+        if constexpr (G == 8) reinterpret_cast<uint2*>(qr)[g] = make_uint2(w[0], w[1]);
+        else reinterpret_cast<uint32_t*>(qr)[g] = w[0];
+    }
+}
+
+// rows of any length, alignment and distance: two passes over the row, the second from cache
+template <typename T>
+__global__ void __launch_bounds__(QT) quantize_any_kernel(const T* x, long long ldx, int K, signed char* q, long long ldq, float* scale)
+{
+    grid_release();
+    const T* xr = x + (size_t) blockIdx.x * ldx;
+    uint32_t m = 0;
+    for (int k = threadIdx.x; k < K; k += QT) m = max(m, __float_as_uint(to_f32(xr[k])) & 0x7fffffffu);
+    const float s = __fdiv_rn(block_amax(m), 127.0f);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
     signed char* qr = q + (size_t) blockIdx.x * ldq;
-    for (int k = threadIdx.x; k < K; k += 256)
-        qr[k] = (signed char) (s > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(to_f32(xr[k]), s)))) : 0);
+    for (int k = threadIdx.x; k < K; k += QT) qr[k] = (signed char) quantise(to_f32(xr[k]), s);
+}
+
+template <typename T>
+void launch_quantize(const void* xv, long long ldx, int rows, int K, signed char* q, long long ldq, float* scale, cudaStream_t st)
+{
+    constexpr int G = 16 / sizeof(T);
+    const T* x = static_cast<const T*>(xv);
+    const int nv = (K / G + QT - 1) / QT;
+    if (K % G || ldx % G || !dense_aligned(x) || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || nv > 8)
+        quantize_any_kernel<T><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
+    else if (nv == 1) quantize_kernel<T, 1><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
+    else if (nv == 2) quantize_kernel<T, 2><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
+    else if (nv == 3) quantize_kernel<T, 3><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
+    else if (nv == 4) quantize_kernel<T, 4><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
+    else quantize_kernel<T, 8><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
 }
 
 }  // namespace
@@ -48,9 +125,9 @@ extern "C" int glmx_quantize_rows(const void* x, int x_dtype, long long ldx, int
     if (rows == 0) return GLMX_OK;
     if (!x || !q || !scale) return dense_fail(GLMX_E_ARG, "glmx_quantize_rows: null argument");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (x_dtype == GLMX_F32) quantize_kernel<<<rows, 256, 0, st>>>(static_cast<const float*>(x), ldx, K, q, ldq, scale);
-    else if (x_dtype == GLMX_F16) quantize_kernel<<<rows, 256, 0, st>>>(static_cast<const __half*>(x), ldx, K, q, ldq, scale);
-    else quantize_kernel<<<rows, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ldx, K, q, ldq, scale);
+    if (x_dtype == GLMX_F32) launch_quantize<float>(x, ldx, rows, K, q, ldq, scale, st);
+    else if (x_dtype == GLMX_F16) launch_quantize<__half>(x, ldx, rows, K, q, ldq, scale, st);
+    else launch_quantize<__nv_bfloat16>(x, ldx, rows, K, q, ldq, scale, st);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? GLMX_OK : dense_cuda_fail(e, "glmx_quantize_rows: launch");
 }
