@@ -359,6 +359,11 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
 __device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -478,12 +483,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int BN = a.BN, NST = pair_stages(BN), STAGE = pair_stage(BN);
-    if (tid == 0)
+    if (warp == 0)
     {
-        for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&tfull[s], 1); mbar_init(&tempty[s], 2 * PAIR_EPI); }
-        s_abort = 0;
+        if (lane < NST) { mbar_init(&full[lane], 1); mbar_init(&empty[lane], 1); }
+        if (lane < 2) { mbar_init(&tfull[lane], 1); mbar_init(&tempty[lane], 2 * PAIR_EPI); }
+        if (lane == 0) s_abort = 0;
         fence_barrier_init();
+    }
+    else if (warp == 2 && lane == 0)
+    {
+        prefetch_map(&maps.a[0]);
+        prefetch_map(&maps.b[EPI == EPI_GATED ? (int) rank : 0]);
     }
     if (warp == 1) tc_alloc<2>(&tmem_slot, 512);
     tc_before();
@@ -770,12 +780,21 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
     };
     auto load_x = [&](int s, int sg, int c) { tma_load_2d(smem + (size_t) s * STAGE + 16384, &maps.x[sg], c, ttile * NT, &full[s]); };
     const int ahead = nk < NST ? nk : NST;                 // stages that need no wait
+    if (warp == 0)
+    {
+        if (lane < NST) { mbar_init(&full[lane], 1); mbar_init(&empty[lane], 1); }
+        if (lane == COLS_STAGES_MAX) { mbar_init(&tfull, 1); s_abort = 0; }
+        fence_barrier_init();
+        __syncwarp();
+    }
+    else if (warp == 2 && lane == 0)
+    {
+        prefetch_map(&maps.w[0]);
+        prefetch_map(&maps.x[0]);
+        if (EPI == EPI_GATED) prefetch_map(&maps.w[1]);
+    }
     if (tid == 0)
     {
-        for (int s = 0; s < NST; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        mbar_init(&tfull, 1);
-        s_abort = 0;
-        fence_barrier_init();
         // the first loads do not wait for the rest of the CTA
         if (!a.prefetch) grid_wait();
         for (int i = 0, sg = seg, c = kc; i < ahead; ++i, step(sg, c)) load_w(i, sg, c);
@@ -988,7 +1007,7 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
 //     (the loads of A then bind) or its share of the weights' stream from memory, a round at least the epilogue of a tile, plus the
 //     start and the last tile's epilogue.
 //   cols_kernel: rounds of clusters, each CTA 3.4 us and 0.018 per token column (start, join) plus its stages on the tensor
-//     cores; or the stream of all tiles' weights from memory (5.9 TB/s), or of all stages from L2 (9 TB/s).
+//     cores; or the stream of all tiles' weights from memory (5.9 TB/s from 130 CTAs on), or of all stages from L2 (9 TB/s).
 // E.g. (measured, us, cols / pair 64 / 128 / 256): feed-forward at H = 6144, I = 1536 of 1 row 18 / 54 / 38 / 45, of 200 rows 29 / 33
 // / 31 / 48, of 512 48 / 53 / 37 / 49, of 4096 263 / 272 / 184 / 163; int8 1024 x 1024 of 48 rows 4.6 / 5.8 / 6.4 / 8.8, of 512 9.5
 // / 5.8 / 6.7 / 9.3.
@@ -1047,10 +1066,11 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms, const ColsC
     {
         const int room = cap.n[one][s];
         if (room < 1) continue;
+        const double ctas = (double) (tiles < room ? tiles : room) * s;              // at once
         const double rounds = (double) ((tiles + room - 1) / room), own = 3.4 + 0.018 * p.NT;
         const double tc = rounds * (own + (double) ((nk + s - 1) / s) * (0.2 + 0.0016 * p.NT));
-        const double hbm = own + (double) p.mtiles * nk * 16384 / 5.9e6, l2 = own + (double) tiles * nk * stage / 9.0e6;
-        const double most = tc > hbm ? tc : hbm, us = (most > l2 ? most : l2) + 0.05 * s;
+        const double hbm = own + (double) p.mtiles * nk * 16384 / (5.9e6 * (ctas < 130 ? ctas / 130 : 1.0)), l2 = own + (double) tiles * nk * stage / 9.0e6;
+        const double most = tc > hbm ? tc : hbm, us = (most > l2 ? most : l2) + 0.02 * s;
         if (us < p.us - 1e-9) { p.us = us; p.splits = s; }
     }
     (void) sms;
@@ -1072,19 +1092,24 @@ cudaError_t cols_capacity(int dev, const ColsCapacity** out)
     if (!ready[dev])
     {
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, COLS_SMEM1);
+        if (err == cudaSuccess)
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         for (int i = 0; i < 2; ++i)
             for (int s = 1; s <= 8 && err == cudaSuccess; ++s)
             {
                 cudaLaunchConfig_t cfg = {};
                 cfg.gridDim = dim3(s, 1024);
                 cfg.blockDim = dim3(COLS_THREADS);
-                cfg.dynamicSmemBytes = i ? COLS_SMEM1 : COLS_SMEM2;
+                cfg.dynamicSmemBytes = COLS_SMEM1;
                 cudaLaunchAttribute attr[1];
                 attr[0].id = cudaLaunchAttributeClusterDimension;
                 attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
                 cfg.attrs = attr;
                 cfg.numAttrs = 1;
                 err = cudaOccupancyMaxActiveClusters(&cap[dev].n[i][s], kernel, &cfg);
+                // the occupancy calculator counts one CTA an SM for every kernel that allocates tensor memory; two of the smaller kind do
+                // run at once (seen by their clocks and SM numbers)
+                if (i == 0) cap[dev].n[i][s] *= 2;
             }
         if (err != cudaSuccess) return err;
         ready[dev] = true;
