@@ -1052,7 +1052,7 @@ struct ColsCapacity
 
 // Tokens per tile: all of them up to 256, else equal tiles. Splits of K: at most 8 (the portable cluster size), each CTA with at least
 // two stages.
-inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms, const ColsCapacity& cap)
+inline ColsPlan cols_plan(int M, int N, bool gated, int nk, const ColsCapacity& cap)
 {
     ColsPlan p;
     p.ttiles = (M + 255) / 256;
@@ -1062,7 +1062,7 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms, const ColsC
     const long long tiles = (long long) p.ttiles * p.mtiles;
     p.splits = 1;
     p.us = 1e30;
-    for (int s = 1; s <= 8 && (s == 1 || 2 * s <= nk); ++s)
+    for (int s = 1; s <= 8 && (s == 1 || 2 * s <= nk) && tiles <= 65535; ++s)   // (tiles are the grid's y dimension)
     {
         const int room = cap.n[one][s];
         if (room < 1) continue;
@@ -1073,7 +1073,6 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, int sms, const ColsC
         const double most = tc > hbm ? tc : hbm, us = (most > l2 ? most : l2) + 0.02 * s;
         if (us < p.us - 1e-9) { p.us = us; p.splits = s; }
     }
-    (void) sms;
     const int room = one ? COLS_SMEM1 : COLS_SMEM2, per = (nk + p.splits - 1) / p.splits;
     p.stages = (room - 2048) / stage;
     if (p.stages > COLS_STAGES_MAX) p.stages = COLS_STAGES_MAX;
@@ -1161,7 +1160,7 @@ cudaError_t launch_product(int dtype, const Product& pr, int nseg, int K, bool p
     const ColsCapacity* cap;
     const cudaError_t err = cols_capacity<I8, W_MN, EPI>(dev, &cap);
     if (err != cudaSuccess) return err;
-    const ColsPlan c = cols_plan(pr.e.M, pr.e.N, EPI == EPI_GATED, nk, sms, *cap);
+    const ColsPlan c = cols_plan(pr.e.M, pr.e.N, EPI == EPI_GATED, nk, *cap);
     const PairPlan p = pair_plan(1, &pr.e, EPI == EPI_GATED, !W_MN, nk, sms);
     if (c.us <= p.us) return launch_cols<I8, W_MN, EPI>(dtype, pr, nseg, K, c, prefetch, st);
     return launch_pair<I8, false, W_MN, EPI>(dtype, 1, &pr, nseg, K, p.BN, st);

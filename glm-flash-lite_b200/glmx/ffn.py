@@ -188,8 +188,9 @@ class _GatedFFNFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_ffn is differentiable once (create_graph is not supported)")
         x2, h, pq = ctx.saved_tensors[:3]            # (and an error here where a weight was changed in between)
         return (*ctx.ffn.backward(dy, (x2, h, pq), ctx.needs_input_grad), None)
 

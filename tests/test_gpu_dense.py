@@ -253,6 +253,14 @@ def test_ffn_autograd_forms(dev):
     assert rel_rms(w.grad, ref[2] + ref[3]) <= 3 * r(BF)     # one more rounding: the sum of the two
     with torch.no_grad():
         assert gated_ffn(xs, wgp, wu, wd).grad_fn is None
+    # a second derivative is refused, and so is a weight that changed after the forward call
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(gated_ffn(xs, wgp, wu, wd).sum(), xs, create_graph=True)
+    y = gated_ffn(xs, wgp, wu, wd)
+    with torch.no_grad():
+        wgp.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
 
 
 def test_ffn_infinite_and_nan_rows_stay_in_their_rows(dev):
