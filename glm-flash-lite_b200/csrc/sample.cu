@@ -9,7 +9,7 @@
 // Few logits matter as a rule. The largest logit of each thread's share is known from the load: where k of these lie above a bin's
 // edge, the top k logits do. What lies above is gathered (at most 512 logits, else the general way) and sorted in one
 // CTA, which finishes the row; without a top-k the same is done where the gathered weights reach top_p.
-// Otherwise the threshold is found by a histogram of 1024 bins of m - l (for top-p of the interval of exponents in which it
+// Otherwise the threshold is found by a histogram of 512 bins of m - l (for top-p of the interval of exponents in which it
 // falls, known from the pass that sums the weights), whose bin is gathered and sorted or, where it holds more than 512 logits, narrowed by histograms over
 // keys (order-preserving integers); and the pick by running sums over the row: the CTA, the warp, then the lane in whose
 // run the target falls.
@@ -32,7 +32,7 @@ struct SampleArgs
     void* ids; int ids64;
 };
 
-constexpr int ST = 512, SBINS = 1024, SLIST = 512, SRANKS = 8;
+constexpr int ST = 512, SBINS = ST, SLIST = 512, SRANKS = 8;
 constexpr int SLICE_MAX = GLMX_SAMPLE_MAX_VOCAB / SRANKS;  // 49152 logits: 192 KB
 constexpr int NPV = 4;                                     // weights are also summed down to these exponents: a histogram then covers one interval
 __device__ constexpr float PV[NPV + 1] = { 4.0f, 6.5f, 9.0f, 12.0f, 30.6f };   // (exp(-30.5) = 2^-44: what lies further down weighs nothing)
@@ -111,17 +111,15 @@ __device__ __forceinline__ uint32_t dsmem_map(const void* p, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
     return r;
 }
-__device__ __forceinline__ u64 dsmem_ld(const void* p, uint32_t rank)
-{
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(dsmem_map(p, rank)) : "memory");
-    return v;
-}
-// the pair of words at p in each of nc CTAs, all loads in flight at once
-__device__ __forceinline__ void dsmem_ld_all(const void* p, int nc, u64 (&v)[SRANKS])
+// the word at p in each of nc CTAs, all loads in flight at once
+__device__ __forceinline__ void dsmem_ld_all(const uint32_t* p, int nc, uint32_t (&v)[SRANKS])
 {
 #pragma unroll
-    for (int r = 0; r < SRANKS; ++r) v[r] = r < nc ? dsmem_ld(p, r) : 0ull;
+    for (int r = 0; r < SRANKS; ++r)
+    {
+        v[r] = 0;
+        if (r < nc) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[r]) : "r"(dsmem_map(p, r)) : "memory");
+    }
 }
 __device__ __forceinline__ uint32_t dsmem_add(const void* p, uint32_t rank, uint32_t v)
 {
@@ -390,8 +388,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         return t >= S ? S - 1 : t;
     };
     // bins of m - l (monotone in l); what lies beyond the span is in the last one
-    auto bin_scale = [&](float span) { return span > 0.0f ? 1023.9f / span : 0.0f; };
-    auto bin_at = [&](float l, float scale) { return l == mx ? 0 : (int) fminf((mx - l) * scale, 1023.0f); };
+    auto bin_scale = [&](float span) { return span > 0.0f ? (SBINS - 0.1f) / span : 0.0f; };
+    auto bin_at = [&](float l, float scale) { return l == mx ? 0 : (int) fminf((mx - l) * scale, SBINS - 1.0f); };
     // f(logit, place in the slice) of this thread's share, the groups that it loaded
     auto each = [&](auto f) {
         for (int j = tid * G; j < n; j += ST * G)
@@ -417,19 +415,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         for (int i = 0; i < ST / 32; ++i) all += sh.warp[i];
         return all;
     };
-    // the bin (of this thread's two) in which the running sum of v0, v1 reaches need
-    auto crossing = [&](u64 v0, u64 v1, u64 upto, u64 need, uint32_t c0, uint32_t c1) {
-        const u64 before = upto - v0 - v1;
-        if (before < need && upto >= need)
-        {
-            const bool second = before + v0 < need;
-            Found f;
-            f.bin = 2 * tid + second;
-            f.above = before + (second ? v0 : 0);
-            f.in = second ? v1 : v0;
-            f.cnt_in = second ? c1 : c0;
-            sh.found = f;
-        }
+    // the bin (a thread's each) in which the running sum of v reaches need
+    auto crossing = [&](u64 v, u64 upto, u64 need, uint32_t cnt) {
+        if (upto - v < need && upto >= need) sh.found = Found{ tid, upto - v, v, cnt };
         __syncthreads();
         return sh.found;
     };
@@ -458,16 +446,13 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         if (mine_max != NONE) atomicAdd(&sh.maxima[bin_at(mine_max, scale)], 1u);
         if (tid == 0) { sh.n_list = 0; sh.found.bin = -1; }
         sync();
-        uint32_t c0 = 0, c1 = 0, all32;
-        {
-            u64 c[SRANKS];
-            dsmem_ld_all(&sh.maxima[2 * tid], NC, c);
+        uint32_t cnt = 0, all32, c[SRANKS];
+        dsmem_ld_all(&sh.maxima[tid], NC, c);
 #pragma unroll
-            for (int r = 0; r < SRANKS; ++r) { c0 += (uint32_t) c[r]; c1 += (uint32_t) (c[r] >> 32); }
-        }
-        const uint32_t cs = block_scan(c0 + c1, sh.warp32, all32);
+        for (int r = 0; r < SRANKS; ++r) cnt += c[r];
+        const uint32_t upto32 = block_scan(cnt, sh.warp32, all32);
         const uint32_t want = by_k ? (uint32_t) k : min(all32, (uint32_t) TRY);
-        const int edge = crossing(c0, c1, cs, want, c0, c1).bin;   // -1: fewer maxima than k
+        const int edge = crossing(cnt, upto32, want, cnt).bin;   // -1: fewer maxima than k
         // gathered: what lies up to the edge (and a rounding more), straight into CTA 0's list, so that the others are done once their
         // shares are in; with top-p alone, all weights are summed as well
         const float floor_l = edge >= 0 ? bin_floor(edge, scale) : INF;
@@ -545,35 +530,27 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         });
         __syncthreads();
         // the copies into one
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
         {
-            const int q = 2 * tid + i;
-            const u64 t = (u64) h.lo[0][q] + h.lo[1][q] + h.lo[2][q] + h.lo[3][q];
-            h.lo[0][q] = (uint32_t) t;
-            h.hi[q] += (uint32_t) (t >> 32);
+            const u64 t = (u64) h.lo[0][tid] + h.lo[1][tid] + h.lo[2][tid] + h.lo[3][tid];
+            h.lo[0][tid] = (uint32_t) t;
+            h.hi[tid] += (uint32_t) (t >> 32);
         }
         sync();
-        // bins 2 tid and 2 tid + 1 of all CTAs
-        u64 v0 = 0, v1 = 0, c[SRANKS], hi[SRANKS];
-        uint32_t c0 = 0, c1 = 0;
-        dsmem_ld_all(&h.lo[0][2 * tid], NC, c);
-        dsmem_ld_all(&h.hi[2 * tid], NC, hi);
+        // bin tid of all CTAs
+        u64 v = 0, all;
+        uint32_t cnt = 0, c[SRANKS], hi[SRANKS];
+        dsmem_ld_all(&h.lo[0][tid], NC, c);
+        dsmem_ld_all(&h.hi[tid], NC, hi);
 #pragma unroll
-        for (int r = 0; r < SRANKS; ++r)
-        {
-            v0 += (c[r] & 0xffffffffu) + (hi[r] << 32);
-            v1 += (c[r] >> 32) + (hi[r] >> 32 << 32);
-        }
+        for (int r = 0; r < SRANKS; ++r) v += (u64) hi[r] << 32 | c[r];
         if (counts)
         {
-            dsmem_ld_all(&h.cnt[2 * tid], NC, c);
+            dsmem_ld_all(&h.cnt[tid], NC, c);
 #pragma unroll
-            for (int r = 0; r < SRANKS; ++r) { c0 += (uint32_t) c[r]; c1 += (uint32_t) (c[r] >> 32); }
+            for (int r = 0; r < SRANKS; ++r) cnt += c[r];
         }
-        u64 all;
-        const u64 upto = block_scan(v0 + v1, sh.warp, all);
-        return crossing(v0, v1, upto, need, mass ? c0 : (uint32_t) v0, mass ? c1 : (uint32_t) v1);
+        const u64 upto = block_scan(v, sh.warp, all);
+        return crossing(v, upto, need, mass ? cnt : (uint32_t) v);
     };
     // id order over the cluster: this CTA's share of a sum, the sums before it and of all
     auto spread = [&](u64 mine, u64& before, u64& all) {
@@ -688,7 +665,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
         f.cnt_in = cnt;
         while (lo < hi)
         {
-            const int s = max(0, 32 - __clz(hi - lo) - 10);
+            const int s = max(0, 32 - __clz(hi - lo) - 9);       // 512 bins
             const float lo_l = of_key<T>(lo), hi_l = of_key<T>(hi);
             f = histogram(mass, true, need - above, [&](float l) { return l >= lo_l && l <= hi_l ? (int) ((hi - key_of<T>(l)) >> s) : -1; });
             above += f.above;
@@ -772,7 +749,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
             }
         need -= above;
         const float scale = bin_scale(width * T0);
-        auto bin = [&](float l) { return l >= low && l < below ? (int) fminf((top - l) * scale, 1023.0f) : -1; };
+        auto bin = [&](float l) { return l >= low && l < below ? (int) fminf((top - l) * scale, SBINS - 1.0f) : -1; };
         const Found f = histogram(true, false, need, bin);
         auto in_bin = [&](float l, int j) { return l != NONE && bin(l) == f.bin && kept(l, j); };
         if (!resolve(true, need, f, in_bin)) narrow(true, need, f, in_bin);
