@@ -144,13 +144,20 @@ class MoELayer:
 
     def forward(self, x: torch.Tensor, sel: torch.Tensor, w: torch.Tensor, mode: int = _lib.MODE_EXACT,
                 out: torch.Tensor | None = None, out_dtype=torch.float32, accumulate: bool = False,
-                stream=None, events=None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+                stream=None, events=None, workspace: torch.Tensor | None = None, dense_shared=None) -> torch.Tensor:
         """out [ntok, H] = sum over each token's picks of w * expert(x) (+ shared expert).
         mode: 1 EXACT (default: fp16 codebook weights, fp32 accumulation, the reference's EXACT arithmetic), 2 I16
         (bit-identical to the reference's I16 kernel; int16 activations, outside the 2e-3 bar at H=6144).
         events: optional list of _lib.PHASES torch.cuda.Event recorded between the kernels on the launching stream.
         workspace: a uint8 CUDA tensor of at least workspace_bytes(ntok, topk) to use instead of the layer's own (calls
-        that may run at the same time on different streams need workspaces of their own)."""
+        that may run at the same time on different streams need workspaces of their own).
+        dense_shared: a GatedFFN (an unquantised shared expert over the same H) whose output for x, rounded to its dtype, is
+        added to out; out must be fp32 or of its dtype."""
+        if dense_shared is not None:
+            if dense_shared.H != self.H or dense_shared.device != self.device:
+                raise ValueError("dense_shared must have the layer's hidden size and device")
+            if (out_dtype if out is None else out.dtype) not in (torch.float32, dense_shared.dtype):
+                raise TypeError(f"out must be fp32 or {dense_shared.dtype} with dense_shared")
         x = x.contiguous(); sel = sel.contiguous(); w = w.contiguous()
         ntok = x.shape[0]
         topk = sel.shape[1] if sel.dim() == 2 else 0
@@ -176,6 +183,9 @@ class MoELayer:
         check(self.lib.glmx_moe_forward_timed(self.h, x.data_ptr(), _dt(x), ntok, sel.data_ptr(), _dt(sel), w.data_ptr(),
                                               _dt(w), topk, int(mode), out.data_ptr(), _dt(out), int(bool(accumulate)),
                                               ws.data_ptr(), ws.numel(), _stream_ptr(stream), ev))
+        if dense_shared is not None:
+            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream()):
+                dense_shared.forward(x.to(dense_shared.dtype), out=out, accumulate=True)
         return out
 
     def forward_hc(self, x: torch.Tensor, sel: torch.Tensor, w: torch.Tensor, hc_x: torch.Tensor, post: torch.Tensor,

@@ -552,8 +552,7 @@ def test_block_head_and_sampling_together(dev):
 
     def step():
         sel, w, _ = router(x)
-        out = layer.forward(x, sel, w)
-        ffn(x, out=out, accumulate=True)
+        out = layer.forward(x, sel, w, dense_shared=ffn)
         logits = lin((out + x.float()).half())
         return out, logits, sample(logits, u, temperature=0.8, top_k=40, top_p=0.95)
 
@@ -562,6 +561,13 @@ def test_block_head_and_sampling_together(dev):
     y, bound = y_bound(x, ffn.w_gate, ffn.w_up, ffn.w_down, 10.0, HF, F32)
     base = layer.forward(x, sel, w)
     assert bool(((out.double() - base.double() - y).abs() <= bound + r(F32) * (out.double().abs() + bound)).all())
+    assert torch.equal(out, ffn(x, out=base.clone(), accumulate=True))
+    assert torch.equal(layer.forward(x.float(), sel, w, dense_shared=ffn, stream=torch.cuda.current_stream()), out)
+    with pytest.raises(ValueError):
+        layer.forward(x, sel, w, dense_shared=GatedFFN(ffn.w_gate[:, :256].contiguous(), ffn.w_up[:, :256].contiguous(),
+                                                       ffn.w_down[:256].contiguous()))
+    with pytest.raises(TypeError):
+        layer.forward(x, sel, w, out_dtype=BF, dense_shared=ffn)
     assert ids.tolist() == sample_ref(logits, u, 0.8, 40, 0.95, 0.0)
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):
