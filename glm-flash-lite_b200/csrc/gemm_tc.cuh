@@ -383,7 +383,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity)
     if ((threadIdx.x & 31) == 0)
     {
         ok = false;
-        for (int i = 0; i < 64 && !(ok = mbar_try_wait(bar, parity)); ++i) __nanosleep(64);
+        for (int i = 0; i < 256 && !(ok = mbar_try_wait(bar, parity)); ++i) __nanosleep(64);
         if (!ok) ok = mbar_wait_bounded(bar, parity);
     }
     return __shfl_sync(0xffffffffu, (int) ok, 0) != 0;
@@ -449,7 +449,7 @@ struct PairArgs
     int nprob;                  // products in the launch (the weights' gradients: three); problem p has maps a[p], b[p], epilogue e[p]
     int nseg;                   // 1; 2: one product whose sum runs over a[0] b[0] and a[1] b[1]
     int K, bk;                  // inputs per segment, and per stage (128 bytes)
-    int BN;                     // columns per tile: 64 (weights K-major only), 128 or 256
+    int BN;                     // columns per tile: 128 or 256; with K-major weights also 64 or 192
     int mt[MAXPROB], nt[MAXPROB], tile0[MAXPROB + 1];    // tiles along M and N, and the first tile of each problem
     uint32_t idesc;
     int* err;
@@ -620,8 +620,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 const int row0 = m * 2 * PAIR_BM + (int) rank * PAIR_BM + 32 * q;
                 const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
                 const float xs = EPI == EPI_I8 && row0 + lane < e.M ? e.xs[row0 + lane] : 0.0f;
-                const int wide = f32 ? 32 : 64, share = max(wide, BN / 2);   // (of a narrow tile, one warp takes all columns)
-                for (int c = half * share; c < min(BN, (half + 1) * share); c += wide)
+                const int wide = f32 ? 32 : 64;
+                for (int c = half * wide; c < BN; c += 2 * wide)
                 {
                     const int n0 = n * BN + c;
                     if (lane == 0) tma_store_read();                   // the tile before has been read
@@ -1003,7 +1003,7 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
 }
 
 // Microseconds of a launch by a simple model of what was measured on a B200; the kernel and its tiling are those of the least.
-//   pair_kernel: rounds of tiles over the pairs, each stage (128 bytes of K) 0.345 us at 256 columns, 0.20 at 128, 0.16 at 64
+//   pair_kernel: rounds of tiles over the pairs, each stage (128 bytes of K) 0.345 us at 256 columns, 0.27 at 192, 0.20 at 128, 0.16 at 64
 //     (the loads of A then bind) or its share of the weights' stream from memory, a round at least the epilogue of a tile, plus the
 //     start and the last tile's epilogue.
 //   cols_kernel: rounds of clusters, each CTA 3.4 us and 0.018 per token column (start, join) plus its stages on the tensor
@@ -1017,20 +1017,21 @@ struct PairPlan
     double us;
 };
 
-inline PairPlan pair_plan(int nprob, const Epi* e, bool gated, bool narrow_ok, int nk, int sms)
+inline PairPlan pair_plan(int nprob, const Epi* e, bool gated, bool kmajor, int nk, int sms)
 {
     PairPlan best{ 256, 1e30 };
-    for (int BN = 256; BN >= (narrow_ok ? 64 : 128); BN /= 2)
+    for (int BN = 256; BN >= 64; BN -= 64)
     {
+        if (BN % 128 && !kmajor) continue;                 // MN-major boxes are 64 columns, two halves of a tile
         long long tiles = 0;
         const int width = gated ? BN / 2 : BN;
         for (int i = 0; i < nprob; ++i) tiles += (long long) ((e[i].M + 255) / 256) * ((e[i].N + width - 1) / width);
         const double rounds = (double) ((tiles + sms / 2 - 1) / (sms / 2));
-        double step = BN == 256 ? 0.345 : BN == 128 ? 0.20 : 0.16;
+        double step = BN == 256 ? 0.345 : BN == 192 ? 0.27 : BN == 128 ? 0.20 : 0.16;
         const double active = (double) (tiles < sms / 2 ? tiles : sms / 2), stream = active * BN * 128 / ((e[0].M + 255) / 256) / 5.4e6;
         if (nprob == 1 && stream > step) step = stream;
-        const double main = nk * step, drain = BN == 256 ? 2.6 : BN == 128 ? 2.0 : 1.2;
-        const double us = (BN == 256 ? 6.6 : BN == 128 ? 5.2 : 4.4) + rounds * (main > drain ? main : drain);
+        const double main = nk * step, drain = BN == 256 ? 2.6 : BN == 192 ? 2.4 : BN == 128 ? 2.0 : 1.2;
+        const double us = (BN == 256 ? 6.6 : BN == 192 ? 6.0 : BN == 128 ? 5.2 : 4.4) + rounds * (main > drain ? main : drain);
         if (us < best.us - 1e-9) best = { BN, us };
     }
     return best;
