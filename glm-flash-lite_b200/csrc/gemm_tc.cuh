@@ -421,22 +421,33 @@ __device__ __forceinline__ void copy_rows(const Epi& e, const uint4* stg, int ro
     const uint32_t* w = reinterpret_cast<const uint32_t*>(stg);
     const int rows = min(32, e.M - row0), cols = min(wide, e.N - n0);
     if (cols <= 0) return;
-    for (int r = 0; r < rows; ++r)
+    const size_t first = (size_t) row0 * e.ldy + n0;
+    // eight rows at a time, their loads and exchanges before their stores
+    for (int r0 = 0; r0 < rows; r0 += 8)
     {
-        const uint32_t v = w[(r * 8 + ((lane >> 2) ^ (r & 7))) * 4 + (lane & 3)];
+        uint32_t v[8], next[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = w[((r0 + i) * 8 + ((lane >> 2) ^ i)) * 4 + (lane & 3)];
         if (wide == 32)
         {
-            if (lane < cols) static_cast<uint32_t*>(e.y)[(size_t) (row0 + r) * e.ldy + n0 + lane] = v;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (r0 + i < rows && lane < cols) static_cast<uint32_t*>(e.y)[first + (size_t) (r0 + i) * e.ldy + lane] = v[i];
             continue;
         }
-        uint16_t* d = static_cast<uint16_t*>(e.y) + (size_t) (row0 + r) * e.ldy + n0;
-        const bool odd = (reinterpret_cast<uintptr_t>(d) & 2) != 0;
-        const uint32_t next = __shfl_down_sync(0xffffffffu, v, 1);
-        const uint32_t word = odd ? (v >> 16) | (next << 16) : v;
-        const int c = 2 * lane + odd;                      // the word's first column
-        if (c + 1 < cols) *reinterpret_cast<uint32_t*>(d + c) = word;
-        else if (c < cols) d[c] = (uint16_t) word;
-        if (odd && lane == 0) d[0] = (uint16_t) v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) next[i] = __shfl_down_sync(0xffffffffu, v[i], 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            uint16_t* d = static_cast<uint16_t*>(e.y) + first + (size_t) (r0 + i) * e.ldy;
+            const bool odd = (reinterpret_cast<uintptr_t>(d) & 2) != 0, in = r0 + i < rows;
+            const uint32_t word = odd ? __funnelshift_r(v[i], next[i], 16) : v[i];
+            const int c = 2 * lane + odd;                  // the word's first column
+            if (in && c + 1 < cols) *reinterpret_cast<uint32_t*>(d + c) = word;
+            if (in && c + 1 == cols) d[c] = (uint16_t) word;
+            if (in && odd && lane == 0) d[0] = (uint16_t) v[i];
+        }
     }
 }
 
