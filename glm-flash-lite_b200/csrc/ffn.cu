@@ -6,6 +6,8 @@
 //
 // Gate and up are one product whose tiles hold the same columns of both, so that the activation is its epilogue; dg and du are
 // the epilogue of dh; dx is one sum over both of its products; the weights' gradients are one launch.
+#include <cmath>
+
 #include "gemm_tc.cuh"
 
 namespace glmx {
@@ -18,7 +20,7 @@ long long hidden_pitch(const glmx_ffn* f) { return (f->intermediate + 63) / 64 *
 Epi epi(const glmx_ffn* f, int M, int N)
 {
     Epi e{};
-    e.M = M; e.N = N; e.bf16 = f->dtype == GLMX_BF16; e.vec = 1; e.limit = f->act_limit; e.y_dtype = f->dtype; e.ldy = N;
+    e.M = M; e.N = N; e.bf16 = f->dtype == GLMX_BF16; e.vec = 1; e.limit = std::isinf(f->act_limit) ? 0.0f : f->act_limit; e.y_dtype = f->dtype; e.ldy = N;
     return e;
 }
 

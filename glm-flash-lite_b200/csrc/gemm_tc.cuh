@@ -518,8 +518,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     cluster_sync();
     tc_after();
     const uint32_t tmem = tmem_slot;
-    grid_release();
+    // the next kernel may start once the ones in front of this one are complete: it may read weights before its own wait
     grid_wait();
+    grid_release();
 
     const int pairs = gridDim.x >> 1, first = blockIdx.x >> 1, ntiles = a.tile0[a.nprob];
     const int ksteps = (a.K + a.bk - 1) / a.bk, nk = ksteps * a.nseg;
@@ -839,7 +840,7 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_slot;
-    grid_release();
+    grid_release();                                        // (thread 0 has waited for the kernels in front)
 
     if (warp == 0)
     {

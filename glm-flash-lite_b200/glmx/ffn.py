@@ -1,7 +1,7 @@
 """Gated feed-forward block over dense 16-bit weights (glmx_ffn_forward / glmx_ffn_backward): an unquantised shared expert
 beside MoELayer's trellis experts, or one of the model's dense layers.
 
-    g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L), y = h Wd^T        (L = act_limit; 0: no clamp)
+    g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L), y = h Wd^T        (L = act_limit; 0 or inf: no clamp)
 
 `GatedFFN` is the block at inference, and its forward_train / backward pair the explicit form of a training step (the one
 to capture into a graph); `gated_ffn` is the same as a differentiable function.
@@ -47,6 +47,15 @@ def _rows(t: torch.Tensor, align: int, pitch_of_copy: int = 64) -> torch.Tensor:
     else:
         c.copy_(t)
     return c
+
+
+def dense_check(device=None, stream=None) -> None:
+    """Synchronises the stream and raises GlmxError where a dense operator on the device gave up a bounded wait since the
+    last check (glmx_dense_check)."""
+    index = torch.device("cuda" if device is None else device).index
+    with torch.cuda.device(_current_device() if index is None else index):
+        s = stream if stream is not None else torch.cuda.current_stream()
+        check(_lib.load().glmx_dense_check(int(s.cuda_stream), C.byref(C.c_int())))
 
 
 class GatedFFN:

@@ -286,7 +286,7 @@ GLMX_API int glmx_check_noalloc(const glmx_layer* layer, int ntok, int topk, voi
  * bounded; glmx_dense_check reads their error word. */
 
 /* A gated feed-forward block over dense 16-bit weights: an unquantised shared expert, or a dense layer.
- *   g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L), y = h Wd^T      (L = act_limit; 0: no clamp)
+ *   g = x Wg^T, u = x Wu^T, h = min(silu(g), L) * clamp(u, -L, L), y = h Wd^T      (L = act_limit; 0 or infinity: no clamp)
  * with the layer's clamp (glmx_layer_desc.act_limit). Products are summed in fp32; h is rounded to the block's dtype. */
 typedef struct
 {

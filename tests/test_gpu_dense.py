@@ -23,9 +23,8 @@ def dev():
 @pytest.fixture(autouse=True)
 def no_device_error():
     yield
-    import ctypes as C
-    from glmx import _lib
-    assert _lib.load().glmx_dense_check(int(torch.cuda.current_stream().cuda_stream), C.byref(C.c_int())) == 0
+    from glmx import dense_check
+    dense_check()
 
 
 def r(t):
@@ -231,6 +230,37 @@ def test_ffn_parts_strides_and_empty(dev):
     y, saved = ffn.forward_train(x[:0])
     dx, *dws = ffn.backward(dy[:0], saved)
     assert y.shape == (0, 128) and dx.shape == (0, 128) and all(float(w.abs().max()) == 0 for w in dws)
+
+
+def test_ffn_infinite_limit_is_none(dev):
+    from glmx import GatedFFN
+    x, wg, wu, wd, dy = block(dev, 20, 128, 192, BF, 23)
+    a, b = GatedFFN(wg, wu, wd, act_limit=math.inf), GatedFFN(wg, wu, wd)
+    (ya, sa), (yb, sb) = a.forward_train(x), b.forward_train(x)
+    assert torch.equal(ya, yb) and all(torch.equal(p, q) for p, q in zip(a.backward(dy, sa), b.backward(dy, sb)))
+    # no rows at the limit: zeros are not next to it
+    assert float(GatedFFN(wg, wu, wd, act_limit=1e-30)(torch.zeros_like(x)).abs().max()) == 0.0
+
+
+def test_ffn_in_place_and_offset_outputs(dev):
+    """The output may be the input, and a slice of a larger buffer that is 16-byte aligned; others are refused."""
+    from glmx import GatedFFN, Int8Linear
+    for T in (3, 400):
+        x, wg, wu, wd, _ = block(dev, T, 256, 128, BF, 25)
+        ffn = GatedFFN(wg, wu, wd)
+        want = ffn(x)
+        buf = torch.zeros(T * 256 + 16, device=dev, dtype=BF)
+        out = buf[8:8 + T * 256].view(T, 256)
+        assert torch.equal(ffn(x, out=out), want)
+        with pytest.raises(ValueError):
+            ffn(x, out=buf[1:1 + T * 256].view(T, 256))
+        lin = Int8Linear.from_weight(wg)
+        y = lin(x)
+        buf = torch.zeros(T * 128 + 16, device=dev, dtype=BF)
+        assert torch.equal(lin(x, out=buf[3:3 + T * 128].view(T, 128)), y)
+        assert float(buf[:3].abs().max()) == 0 and float(buf[3 + T * 128:].abs().max()) == 0
+        x2 = x.clone()
+        assert ffn(x2, out=x2) is x2 and torch.equal(x2, want)
 
 
 def test_ffn_autograd_forms(dev):
@@ -523,6 +553,21 @@ def test_sample_rows_and_types(dev):
     assert sample(l[:0], u[:0]).shape == (0,)
 
 
+def test_sample_many_rows(dev):
+    """More rows than one launch's grid takes."""
+    from glmx import sample
+    gen = torch.Generator(device=dev).manual_seed(2)
+    l, u = torch.randn(66000, 5, generator=gen, device=dev), torch.rand(66000, generator=gen, device=dev)
+    k = torch.randint(0, 4, (66000,), generator=gen, device=dev, dtype=torch.int32)
+    got = sample(l, u, top_k=k)
+    w = torch.exp(l.double() - l.double().amax(1, keepdim=True))
+    rank = torch.argsort(torch.argsort(l, dim=1, descending=True), dim=1)
+    w = torch.where((k[:, None] == 0) | (rank < k[:, None]), w, 0.0)
+    c = w.cumsum(1)
+    want = (c > u.double()[:, None] * c[:, -1:]).int().argmax(1)
+    assert torch.equal(got, want)
+
+
 def test_sample_frequencies(dev):
     """Many uniform numbers over one row reproduce its probabilities: counts within 5 standard deviations."""
     from glmx import sample
@@ -636,6 +681,38 @@ def test_streams(dev):
     torch.cuda.synchronize()
     for g in got:
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first call of each operator is captured: nothing of their set-up disturbs the capture."""
+    import subprocess
+    import sys
+    from conftest import PKG
+    code = """
+import sys, torch
+sys.path.insert(0, %r)
+import glmx
+d = 'cuda'
+w, wd, x, dy = (torch.randn(*s, device=d).bfloat16() / 8 for s in ((96, 128), (128, 96), (40, 128), (40, 128)))
+u, ws = torch.rand(40, device=d), torch.rand(96, device=d)
+wq = torch.randint(-9, 9, (96, 128), device=d, dtype=torch.int8)
+ffn, lin = glmx.GatedFFN(w, w, wd), glmx.Int8Linear(wq, ws)
+torch.cuda.synchronize()
+def step():
+    y, saved = ffn.forward_train(x)
+    q, s = glmx.quantize_rows(x)
+    return (y, *ffn.backward(dy, saved), lin.matmul(q, s), glmx.sample(x, u, top_p=0.9))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+glmx.dense_check()
+print('captured')
+""" % PKG
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_first_call_of_a_thread(dev):
