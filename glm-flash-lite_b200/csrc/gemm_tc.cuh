@@ -644,34 +644,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     const int n0 = n * BN + c;
                     if (lane == 0) tma_store_read();                   // the tile before has been read
                     __syncwarp();
-                    for (int d = 0; d < wide; d += 16)
+                    // 32 columns a wait: all 64 at once take the registers that the 8-bit epilogue needs
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
                     {
-                        uint32_t v[16];
-                        tc_ld16(tq + (uint32_t) (c + d), v);
+                        if (f32 && h) break;
+                        uint32_t v[2][16];
+                        tc_ld16(tq + (uint32_t) (c + 32 * h), v[0]);
+                        tc_ld16(tq + (uint32_t) (c + 32 * h + 16), v[1]);
                         tc_wait_ld();
-                        if constexpr (EPI == EPI_I8)
-                        {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
+                        for (int d = 0; d < 2; ++d)
+                        {
+                            if constexpr (EPI == EPI_I8)
                             {
-                                const int col = min(n0 + d + i, e.N - 1);
-                                float f = (float) (int) v[i] * (xs * __ldg(e.ws + col));
-                                if (e.bias) f += __ldg(e.bias + col);
-                                v[i] = __float_as_uint(f);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                {
+                                    const int col = min(n0 + 32 * h + 16 * d + i, e.N - 1);
+                                    float f = (float) (int) v[d][i] * (xs * __ldg(e.ws + col));
+                                    if (e.bias) f += __ldg(e.bias + col);
+                                    v[d][i] = __float_as_uint(f);
+                                }
                             }
-                        }
-                        if (f32)
-                        {
+                            if (f32)
+                            {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) stg[lane * 8 + ((d / 4 + i) ^ (lane & 7))] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                        }
-                        else
-                        {
-                            uint32_t w[8];
+                                for (int i = 0; i < 4; ++i)
+                                    stg[lane * 8 + ((4 * d + i) ^ (lane & 7))] = make_uint4(v[d][4 * i], v[d][4 * i + 1], v[d][4 * i + 2], v[d][4 * i + 3]);
+                            }
+                            else
+                            {
+                                uint32_t w[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) w[i] = pack16(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), bf);
+                                for (int i = 0; i < 8; ++i) w[i] = pack16(__uint_as_float(v[d][2 * i]), __uint_as_float(v[d][2 * i + 1]), bf);
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) stg[lane * 8 + ((d / 8 + i) ^ (lane & 7))] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                                for (int i = 0; i < 2; ++i) stg[lane * 8 + ((4 * h + 2 * d + i) ^ (lane & 7))] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                            }
                         }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
