@@ -1,6 +1,7 @@
 // Sampling (glmx_sample): one cluster of up to 8 CTAs per row, the row's logits held in their shared memory, so that global memory is
 // read once and every further pass runs on chip. One row of 131072 logits is bound by the passes' latency (cluster barriers,
-// block scans), a batch by the exponentials of the rows that keep many tokens.
+// block scans): 13 us in bf16 with all filters. A batch is bound by the passes over the rows that keep many tokens, about 35 us each:
+// 64 rows of 150001 in fp32, some with each filter, 63 to 68 us (512 CTAs, of which 296 run at a time).
 //
 // A weight is w = exp((l - m) / T) <= 1 in fp32, held as the integer floor(w * 2^44): sums of up to 2^19 weights fit 64 bits
 // and do not depend on their order. Equal logits have equal weights, so each filter is a threshold on the logits plus a
