@@ -799,10 +799,10 @@ cudaError_t launch_sample(const SampleArgs& a0, int B, cudaStream_t st)
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     // rows are the grid's y dimension, at most 65535 a launch
-    for (int r = 0; r < B; r += 65535)
+    for (long long r = 0; r < B; r += 65535)
     {
         SampleArgs c = a;
-        const int rows = B - r < 65535 ? B - r : 65535;
+        const int rows = (int) (B - r < 65535 ? B - r : 65535);
         c.logits = static_cast<const T*>(a.logits) + (size_t) r * a.ld;
         c.u += r;
         if (c.temperature) c.temperature += r;

@@ -42,7 +42,8 @@ def _rows(t: torch.Tensor, align: int, pitch_of_copy: int = 64) -> torch.Tensor:
     if R == 1 and inner == 1 and n % align == 0 and t.data_ptr() % 16 == 0:
         return t.as_strided((1, n), (n, 1))
     c = torch.empty((R, (n + pitch_of_copy - 1) // pitch_of_copy * pitch_of_copy), dtype=t.dtype, device=t.device)[:, :n]
-    if t.dtype == torch.int8 and inner == 1 and n % 4 == 0 and pitch % 4 == 0 and t.storage_offset() % 4 == 0 and pitch >= n:
+    if t.dtype == torch.int8 and inner == 1 and n % 4 == 0 and pitch % 4 == 0 and pitch >= n and \
+            t.storage_offset() % 4 == 0 and t.data_ptr() % 4 == 0:
         c.view(torch.int32).copy_(t.view(torch.int32))       # bytes four at a time
     else:
         c.copy_(t)
@@ -168,6 +169,8 @@ class GatedFFN:
         n = x.shape[0]
         if dy2.shape[0] != n:
             raise ValueError("dy must have the forward call's rows")
+        if x.shape[1] != self.H or pq.shape[2] != self.I:
+            raise ValueError("saved must be of a forward_train call of this block")
         H, I, new = self.H, self.I, self._new
         dx = new(dy.shape) if need[0] else None
         dwg = new((I, H)) if need[1] else None
@@ -211,4 +214,6 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
               act_limit: float = 0.0) -> torch.Tensor:
     """The block as a differentiable function of x and its weights (once differentiable; not in a graph capture: see
     GatedFFN.forward_train)."""
+    if not torch.is_grad_enabled():              # a Function's needs_input_grad does not tell: nothing is to be kept
+        return GatedFFN(w_gate, w_up, w_down, act_limit).forward(x)
     return _GatedFFNFunction.apply(x, w_gate, w_up, w_down, float(act_limit))

@@ -122,6 +122,8 @@ class Int8Linear:
             if dt not in _FLOAT:
                 raise TypeError("out_dtype must be fp16, bf16 or fp32")
             out = xq.new_empty((*xq.shape[:-1], self.N), dtype=dt)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError(f"out is {out.dtype}, out_dtype {out_dtype}")
         elif tuple(out.shape) != (*xq.shape[:-1], self.N) or not out.is_contiguous() or out.device != self.device or \
                 out.dtype not in _FLOAT:
             raise ValueError("out must be contiguous fp16 / bf16 / fp32 [..., N] on the weights' device")
@@ -142,4 +144,4 @@ class Int8Linear:
             with ctx:
                 return self(x, out)
         q, s = quantize_rows(x)
-        return self.matmul(q, s, out, self.out_dtype or x.dtype)
+        return self.matmul(q, s, out, (self.out_dtype or x.dtype) if out is None else None)

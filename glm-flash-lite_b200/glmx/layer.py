@@ -152,12 +152,14 @@ class MoELayer:
         workspace: a uint8 CUDA tensor of at least workspace_bytes(ntok, topk) to use instead of the layer's own (calls
         that may run at the same time on different streams need workspaces of their own).
         dense_shared: a GatedFFN (an unquantised shared expert over the same H) whose output for x, rounded to its dtype, is
-        added to out; out must be fp32 or of its dtype."""
+        added to out; out must be fp32 or of its dtype, and share no memory with x."""
         if dense_shared is not None:
             if dense_shared.H != self.H or dense_shared.device != self.device:
                 raise ValueError("dense_shared must have the layer's hidden size and device")
             if (out_dtype if out is None else out.dtype) not in (torch.float32, dense_shared.dtype):
                 raise TypeError(f"out must be fp32 or {dense_shared.dtype} with dense_shared")
+            if out is not None and (out.shape != x.shape or not out.is_contiguous() or out.data_ptr() % 16):
+                raise ValueError("out must be contiguous, 16-byte aligned and of x's shape with dense_shared")
         x = x.contiguous(); sel = sel.contiguous(); w = w.contiguous()
         ntok = x.shape[0]
         topk = sel.shape[1] if sel.dim() == 2 else 0
@@ -168,6 +170,8 @@ class MoELayer:
                 raise ValueError(f"tensor on {t.device}, layer on {self.device}")
         if out is None:
             out = torch.empty((ntok, self.H), dtype=out_dtype, device=self.device)
+        elif dense_shared is not None and out.data_ptr() < x.data_ptr() + x.nbytes and x.data_ptr() < out.data_ptr() + out.nbytes:
+            raise ValueError("out must not overlap x with dense_shared, which reads x after the experts wrote out")
         if workspace is not None:
             if workspace.numel() < self.workspace_bytes(ntok, topk) or workspace.device != self.device:
                 raise ValueError("workspace too small or on another device")

@@ -59,6 +59,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     if not u.is_contiguous():
         u = u.contiguous()
     t, tp, t0 = _param(temperature, torch.float32, B, index, "temperature")
+    if not isinstance(top_k, torch.Tensor):
+        top_k = max(0, min(int(top_k), V))
+    elif top_k.dtype != torch.int32:
+        top_k = top_k.clamp(0, V)                # before the conversion: a larger number keeps its meaning
     k, kp, k0 = _param(top_k, torch.int32, B, index, "top_k")
     p, pp, p0 = _param(top_p, torch.float32, B, index, "top_p")
     m, mp, m0 = _param(min_p, torch.float32, B, index, "min_p")

@@ -781,3 +781,60 @@ def test_refusals_with_device_tensors(dev):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, ffn(x))
+
+
+def test_ffn_without_gradients_is_the_plain_call(dev):
+    """Where gradients are off, leaves that ask for them change nothing: no factors kept, and the call may be captured."""
+    from glmx import GatedFFN, gated_ffn
+    x, wg, wu, wd, _ = block(dev, 64, 512, 1024, BF, 91)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    want = GatedFFN(wg, wu, wd, 3.0)(x)
+    with torch.no_grad():
+        gated_ffn(*leaves, 3.0)
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        y = gated_ffn(*leaves, 3.0)
+        assert torch.cuda.max_memory_allocated() - base <= y.nbytes + 64 * 1024 * 2      # the hidden rows, no more
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cap = gated_ffn(*leaves, 3.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and torch.equal(cap, want) and y.grad_fn is None
+
+
+def test_refusals_of_mixed_up_calls(dev):
+    from glmx import GatedFFN, Int8Linear, MoELayer, quantize_rows, synth
+    x, wg, wu, wd, dy = block(dev, 4, 512, 96, HF, 92)
+    ffn = GatedFFN(wg, wu, wd)
+    small = GatedFFN(wg[:88], wu[:88], wd[:, :88])
+    with pytest.raises(ValueError, match="saved"):
+        ffn.backward(dy, small.forward_train(x)[1])
+    lin = Int8Linear.from_weight(wg)
+    q, s = quantize_rows(x)
+    with pytest.raises(TypeError, match="out_dtype"):
+        lin.matmul(q, s, out=torch.empty(4, 96, device=dev), out_dtype=BF)
+    layer = MoELayer.from_bank(synth.make_bank(512, 256, 8, shared=False, seed=3), device=dev)
+    sel, w = torch.zeros(4, 2, dtype=torch.int32, device=dev), torch.full((4, 2), 0.5, device=dev)
+    sel[:, 1] = 1
+    kept = x.clone()
+    with pytest.raises(ValueError, match="overlap"):
+        layer.forward(x, sel, w, out=x, dense_shared=ffn)
+    with pytest.raises(ValueError, match="aligned"):
+        layer.forward(x, sel, w, out=torch.empty(4 * 512 + 1, device=dev)[1:].view(4, 512), dense_shared=ffn)
+    with pytest.raises(ValueError, match="shape"):
+        layer.forward(x, sel, w, out=torch.empty(5, 512, device=dev), dense_shared=ffn)
+    assert torch.equal(x, kept)
+
+
+def test_sample_top_k_beyond_32_bits(dev):
+    """A top-k larger than the row keeps all of it, however large, as a number and as int64."""
+    from glmx import sample
+    gen = torch.Generator(device=dev).manual_seed(93)
+    logits, u = torch.randn(64, 1000, generator=gen, device=dev), torch.rand(64, generator=gen, device=dev)
+    want = sample(logits, u)
+    for k in ((1 << 32) + 1, 1 << 31):
+        assert torch.equal(sample(logits, u, top_k=k), want)
+        assert torch.equal(sample(logits, u, top_k=torch.full((64,), k, device=dev)), want)
+    assert torch.equal(sample(logits, u, top_k=-5), want) and torch.equal(sample(logits, u, top_k=torch.full((64,), -5, device=dev)), want)
