@@ -24,6 +24,9 @@ inline int dense_cuda_fail(cudaError_t e, const char* what)
 
 inline bool dense_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+int dense_device();                          // the current device, or -1
+int dense_sms(int device);
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }

@@ -993,8 +993,6 @@ struct Mat
 // tensor map of boxes of box_inner x box_rows elements with the 128-byte swizzle
 cudaError_t dense_map(CUtensorMap* m, int dtype, const Mat& t, int box_inner, int box_rows);
 cudaError_t dense_err_ptr(int** p);          // the current device's error word
-int dense_device();                          // the current device, or -1
-int dense_sms(int device);
 
 // One product of the launch: sums over segs (A: tokens, B: weights; GATED: B of seg 0 and 1 are gate and up)
 struct Product

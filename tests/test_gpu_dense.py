@@ -838,3 +838,23 @@ def test_sample_top_k_beyond_32_bits(dev):
         assert torch.equal(sample(logits, u, top_k=k), want)
         assert torch.equal(sample(logits, u, top_k=torch.full((64,), k, device=dev)), want)
     assert torch.equal(sample(logits, u, top_k=-5), want) and torch.equal(sample(logits, u, top_k=torch.full((64,), -5, device=dev)), want)
+
+
+@pytest.mark.parametrize("B", [40, 300, 512, 700])
+def test_sample_rows_with_settings_of_their_own(dev, B):
+    """Every row's pick is the one it gets alone, whatever the order in which a batch's rows are worked on."""
+    from glmx import sample
+    gen = torch.Generator(device=dev).manual_seed(94)
+    V = 20011
+    logits, u = torch.randn(B, V, generator=gen, device=dev) * 3, torch.rand(B, generator=gen, device=dev)
+    row = torch.arange(B, device=dev)
+    temperature = torch.where(row % 7 == 3, 0.0, 0.5 + torch.rand(B, generator=gen, device=dev))
+    top_k = torch.where(row % 3 == 0, 0, torch.where(row % 5 == 0, 5000, 20 + row)).int()
+    top_p = torch.where(row % 4 == 1, 1.0, 0.3 + 0.69 * torch.rand(B, generator=gen, device=dev))
+    got = sample(logits, u, temperature, top_k, top_p, 0.0)
+    for b in range(0, B, 1 if B < 100 else 17):
+        one = sample(logits[b:b + 1], u[b:b + 1], float(temperature[b]), int(top_k[b]), float(top_p[b]), 0.0)
+        assert int(got[b]) == int(one[0]), b
+    assert torch.equal(got, sample(logits, u, temperature, top_k, top_p, torch.zeros(B, device=dev)))
+    perm = torch.randperm(B, generator=gen, device=dev)
+    assert torch.equal(got[perm], sample(logits[perm], u[perm], temperature[perm], top_k[perm], top_p[perm]))
