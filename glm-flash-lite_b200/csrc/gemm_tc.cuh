@@ -4,7 +4,7 @@
 //   pair_kernel: many rows. Persistent CTA pairs (cta_group::2), 256 tokens x 64 to 256 columns per tile, each CTA holding half of
 //     the rows of A and half of the columns of B, so that a byte of shared memory feeds 256 products' worth of either side. Bound by
 //     the tensor cores: a bf16 feed-forward of 4096 rows, H = 2048, I = 8192, 278 us, 1.48 PFLOP/s where a large library
-//     product reaches 1.61; 8-bit, 4096 x 6144 x 12288, 194 us with the rows' quantisation (21). What is lost is the last round of tiles, the
+//     product reaches 1.61; 8-bit, 4096 x 6144 x 12288, 194 us, 3.19 POP/s. What is lost is the last round of tiles, the
 //     start and the last epilogue.
 //   cols_kernel: few rows. The weights are the M operand (128 of their rows per tile), the tokens the N operand (16 .. 256),
 //     and K is split over the CTAs of a cluster, whose partial tiles are added in rank order over distributed shared memory:

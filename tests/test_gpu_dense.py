@@ -858,3 +858,26 @@ def test_sample_rows_with_settings_of_their_own(dev, B):
     assert torch.equal(got, sample(logits, u, temperature, top_k, top_p, torch.zeros(B, device=dev)))
     perm = torch.randperm(B, generator=gen, device=dev)
     assert torch.equal(got[perm], sample(logits[perm], u[perm], temperature[perm], top_k[perm], top_p[perm]))
+
+
+@pytest.mark.parametrize("dt", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+def test_quantize_values_next_to_halves(dev, dt):
+    """Quotients that are k + 1/2, exactly or but for their last bits: each is the fp32 quotient rounded to even, as torch has it."""
+    from glmx import quantize_rows
+    gen = torch.Generator(device=dev).manual_seed(95)
+    R, K = 512, 2048
+    s = torch.rand(R, 1, generator=gen, device=dev) + 0.5
+    s[::2] = torch.randint(1, 1 << 8, (R // 2, 1), generator=gen, device=dev) / 64          # exact halves in 16 bits, too
+    x = (torch.randint(-127, 127, (R, K), generator=gen, device=dev) + 0.5) * s
+    x = x * (1 + torch.randint(-3, 4, (R, K), generator=gen, device=dev) * 2.0 ** -23 * (dt == F32))
+    x[:, 0] = 127 * s[:, 0]
+    x = x.to(dt)
+    scale = x.float().abs().amax(1) / torch.full((R,), 127.0, device=dev)                   # (a scalar divisor would be a reciprocal's product)
+    want = torch.round(x.float() / scale[:, None]).clamp(-127, 127).to(torch.int8)
+    for rows in (slice(None), slice(1)):
+        q, sc = quantize_rows(x[rows])
+        assert torch.equal(q, want[rows]) and torch.equal(sc, scale[rows])
+    for power in (-60, 60):                                                                 # fp32 rows far from 1
+        if dt != HF:
+            q, sc = quantize_rows((x.float() * 2.0 ** power).to(dt))
+            assert torch.equal(q, want) and torch.equal(sc, scale * 2.0 ** power)
