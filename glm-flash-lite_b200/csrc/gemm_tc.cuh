@@ -9,7 +9,7 @@
 //   cols_kernel: few rows. The weights are the M operand (128 of their rows per tile), the tokens the N operand (16 .. 256),
 //     and K is split over the CTAs of a cluster, whose partial tiles are added in rank order over distributed shared memory:
 //     enough CTAs to stream the weights at full bandwidth, one launch, no scratch, the same bits in every run. Bound by that
-//     stream, 5.3 to 7 TB/s, and 5 us around it (the first weights' arrival, the join): 6144 x 6144 bytes 10.5 us for one row,
+//     stream, 5.3 to 7 TB/s, and 5 us around it (the first weights' arrival, the join): 6144 x 6144 bytes 11.4 us for one row,
 //     a feed-forward of 56.6 MB 17.8 us; 65536 x 4096 bytes for 48 rows 55 us.
 //
 // Operands are row-major matrices read by TMA with the 128-byte swizzle: K-major ones [rows][K] in boxes of 128 bytes of K,
