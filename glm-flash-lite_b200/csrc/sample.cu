@@ -61,18 +61,19 @@ __device__ __forceinline__ float of_key(uint32_t k)
 
 struct Weight
 {
-    float m, c;                                            // row maximum, log2(e) / T
+    float h, c;                                            // -(row maximum) / 2, 2 log2(e) / T
     __device__ __forceinline__ void init(float max, float T)
     {
-        m = max;
-        c = (float) fmin(1.4426950408889634 / (double) T, 3e38);
+        h = -0.5f * max;
+        // never 0, also where T is infinite: -inf * 0 would be NaN
+        c = (float) fmax(fmin(2.8853900817779268 / (double) T, 3e38), 0x1p-149);
     }
-    // floor(2^44 2^((l - m) c)). The exponent's rounding moves a weight of 2^-x by x 2^-24 of itself, the exponential by about 2^-22: no more than
-    // fp32 logits carry. -inf gives 0
+    // floor(2^44 2^((l - m) / T log2(e))), of half the difference, which no two finite logits overflow. The exponent's rounding moves a weight of
+    // 2^-x by x 2^-24 of itself, the exponential by about 2^-22: no more than fp32 logits carry. -inf gives 0 at every temperature
     __device__ __forceinline__ u64 operator()(float l) const
     {
         float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((l - m) * c));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(l, 0.5f, h) * c));
         return __float2ull_rd(e * 17592186044416.0f);
     }
 };

@@ -1,0 +1,101 @@
+"""Calls of the dense operators at the edges of what their documentation allows, on the GPU.
+
+Tolerances count roundings. r(t) = torch.finfo(t).eps / 2 is one rounding to t."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda", 0)
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    yield
+    from glmx import dense_check
+    dense_check()
+
+
+def r(t):
+    return torch.finfo(t).eps / 2
+
+
+# ---- sampling ----------------------------------------------------------------------------------------------------------
+
+def picks(logits, u, temperature, top_k, top_p, min_p):
+    """The documented pick, row by row in 64 bits; an infinite temperature is the limit of large ones: equal weights."""
+    out = []
+    for b, l in enumerate(logits.double().cpu()):
+        l = torch.where(l.isnan(), torch.full_like(l, -math.inf), l)
+        m = float(l.max())
+        if m == -math.inf:
+            out.append(-1)
+            continue
+        if math.isinf(temperature):
+            w = (l > -math.inf).double()
+        else:
+            w = torch.exp((l - m) / temperature)
+        order = torch.sort(l, descending=True, stable=True).indices
+        if 0 < top_k < l.numel():
+            order = order[:top_k]
+        ws = w[order]
+        if top_p < 1:
+            before = torch.cumsum(ws, 0) - ws
+            n = max(1, int((before < top_p * ws.sum()).sum()))
+            order, ws = order[:n], ws[:n]
+        ok = ws >= min_p
+        ok[0] = True
+        ids = order[ok].sort().values
+        c = torch.cumsum(w[ids], 0)
+        out.append(int(ids[(c > float(u[b]) * c[-1]).nonzero()[0]]))
+    return out
+
+
+FILTERS = [dict(), dict(min_p=0.25), dict(top_k=5), dict(top_k=700), dict(top_p=0.5), dict(top_k=900, top_p=0.75, min_p=0.25)]
+
+
+@pytest.mark.parametrize("kw", FILTERS, ids=lambda kw: "-".join(kw) + str(kw.get("top_k", "")) or "plain")
+@pytest.mark.parametrize("dt", [F32, BF, HF], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V,start", [(1, 0), (33, 0), (1000, 3), (4099, 1), (20011, 7)])
+def test_sample_infinite_temperature(dev, V, start, dt, kw):
+    """Every logit that may be picked has the same weight, and none that may not has any: masked and NaN ones, and what lies around rows
+    of odd length and start."""
+    from glmx import sample
+    B = 6
+    gen = torch.Generator(device=dev).manual_seed(V + start)
+    wide = torch.full((B, start + V + 5), 100.0, device=dev, dtype=dt)
+    l = wide[:, start:start + V]
+    l.copy_((torch.randn(B, V, generator=gen, device=dev) * 3).to(dt))
+    if V > 1:
+        l[1, torch.rand(V, generator=gen, device=dev) < 0.97] = -math.inf
+        l[2, ::2] = math.nan
+        l[3] = -math.inf
+        l[3, V // 2] = -7.0
+        l[4, 1:] = -math.inf
+    u = torch.rand(B, generator=gen, device=dev)
+    f = dict(top_k=0, top_p=1.0, min_p=0.0) | kw
+    want = picks(l, u, math.inf, **f)
+    assert sample(l, u, temperature=math.inf, **kw).tolist() == want
+    temps = torch.full((B,), math.inf, device=dev)
+    assert sample(l, u, temperature=temps, **kw).tolist() == want
+    temps[::2] = 0.8                                         # each row has its own
+    got = sample(l, u, temperature=temps, **kw).tolist()
+    assert got[1::2] == want[1::2] and got[::2] == picks(l[::2], u[::2], 0.8, **f)
+
+
+def test_sample_logits_further_apart_than_fp32(dev):
+    """The difference of two finite logits may pass the largest fp32 number; the weights of such are as of any others."""
+    from glmx import sample
+    l = torch.tensor([[3e38, -3e38, 0.0, 1e38]], device=dev)
+    for T in (1e38, 3e38, math.inf):
+        for u in (0.05, 0.3, 0.45, 0.55, 0.7, 0.95):
+            assert sample(l, torch.tensor([u], device=dev), temperature=T).tolist() == picks(l, [u], float(torch.tensor(T)), 0, 1.0, 0.0)
