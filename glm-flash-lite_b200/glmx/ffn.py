@@ -82,15 +82,32 @@ class GatedFFN:
             raise ValueError("act_limit must be 0 (none) or positive")
         self._index = w_gate.get_device()
         self._pitch = (self.I + 63) // 64 * 64           # GLMX_FFN_PITCH: elements between hidden rows
-        self.w_gate, self.w_up, self.w_down = self._pack(w_gate), self._pack(w_up), self._pack(w_down)
         self.act_limit = float(act_limit)
+        self._take(*(w.detach() if w.requires_grad else w for w in (w_gate, w_up, w_down)))
+
+    def _take(self, w_gate, w_up, w_down):
+        self.w_gate, self.w_up, self.w_down = self._pack(w_gate), self._pack(w_up), self._pack(w_down)
         self._desc = _lib.Ffn(self.H, self.I, _dt(w_gate), self.w_gate.data_ptr(), self.w_up.data_ptr(),
                               self.w_down.data_ptr(), self.act_limit)
         self._ref = C.byref(self._desc)
 
+    def _bare(self):
+        """The block without its weights."""
+        f = GatedFFN.__new__(GatedFFN)
+        f.__dict__.update(self.__dict__, w_gate=None, w_up=None, w_down=None, _desc=None, _ref=None)
+        return f
+
+    def _with(self, w_gate, w_up, w_down):
+        """The same block over weights of the same shapes, dtype and device."""
+        up = (self.I, self.H)
+        for w, shape in ((w_gate, up), (w_up, up), (w_down, (self.H, self.I))):
+            if w.dtype != self.dtype or w.get_device() != self._index or w.shape != shape:
+                raise ValueError(f"weights must be the block's, {self.dtype} on {self.device}: not {w.dtype} on {w.device}")
+        f = self._bare()
+        f._take(w_gate, w_up, w_down)
+        return f
+
     def _pack(self, w: torch.Tensor) -> torch.Tensor:
-        if w.requires_grad:
-            w = w.detach()
         if w.is_contiguous() and w.data_ptr() % 16 == 0:
             return w
         with torch.cuda.device(self._index):
@@ -197,17 +214,19 @@ class _GatedFFNFunction(torch.autograd.Function):
             raise RuntimeError("gated_ffn: a differentiated call cannot be captured into a graph (an eager graph of the "
                                "same leaves would tie the capture to another stream); capture GatedFFN.forward_train and "
                                "GatedFFN.backward")
-        y, (x2, h, pq) = ffn.forward_train(x)
-        ctx.save_for_backward(x2, h, pq, w_gate, w_up, w_down)
-        ctx.ffn = ffn
+        y, saved = ffn.forward_train(x)
+        ctx.save_for_backward(*saved, w_gate, w_up, w_down)
+        ctx.block = ffn._bare()
         return y
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():
             raise RuntimeError("gated_ffn is differentiable once (create_graph is not supported)")
-        x2, h, pq = ctx.saved_tensors[:3]            # (and an error here where a weight was changed in between)
-        return (*ctx.ffn.backward(dy, (x2, h, pq), ctx.needs_input_grad), None)
+        # the weights as they are unpacked here, not where they were in the forward call: their storage may have moved, or a hook may
+        # have kept them elsewhere (and an error here where a weight was changed in between)
+        *saved, w_gate, w_up, w_down = ctx.saved_tensors
+        return (*ctx.block._with(w_gate, w_up, w_down).backward(dy, saved, ctx.needs_input_grad), None)
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,

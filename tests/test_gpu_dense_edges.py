@@ -99,3 +99,49 @@ def test_sample_logits_further_apart_than_fp32(dev):
     for T in (1e38, 3e38, math.inf):
         for u in (0.05, 0.3, 0.45, 0.55, 0.7, 0.95):
             assert sample(l, torch.tensor([u], device=dev), temperature=T).tolist() == picks(l, [u], float(torch.tensor(T)), 0, 1.0, 0.0)
+
+
+# ---- gated feed-forward ------------------------------------------------------------------------------------------------
+
+def block(dev, T, H, I, dt, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g, device=dev)
+    x = rn(T, H).to(dt)
+    wg, wu = (rn(I, H) * (1.2 / math.sqrt(H))).to(dt), (rn(I, H) * (1.2 / math.sqrt(H))).to(dt)
+    return x, wg, wu, (rn(H, I) / math.sqrt(I)).to(dt), rn(T, H).to(dt)
+
+
+def test_gated_ffn_reads_the_weights_that_were_saved(dev):
+    """The backward pass takes the weights from where autograd has them: kept on the host by a hook, or in a storage that was given
+    back and filled again since the forward call."""
+    from glmx import gated_ffn
+    for T in (5, 300):
+        x, *ws, dy = block(dev, T, 256, 136, BF, 400 + T)
+        for strided in (False, True):
+            def leaves():
+                out = [x.clone().requires_grad_(True)]
+                for w in ws:
+                    w = w.t().contiguous().t() if strided else w.clone()
+                    out.append(w.requires_grad_(True))
+                return out
+            plain = leaves()
+            want = torch.autograd.grad(gated_ffn(*plain, act_limit=2.0), plain, dy)
+            kept = leaves()
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
+                y = gated_ffn(*kept, act_limit=2.0)
+            for w in kept[1:]:
+                w.data.zero_()                               # (unseen by autograd: the hook has the values)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, kept, dy), want))
+            if strided:
+                continue
+            moved = leaves()
+            y = gated_ffn(*moved, act_limit=2.0)
+            sizes = [w.untyped_storage().size() for w in moved[1:]]
+            for w in moved[1:]:
+                w.untyped_storage().resize_(0)
+            junk = [torch.full((n // 2,), math.nan, device=dev, dtype=BF) for n in sizes]
+            for w, n, v in zip(moved[1:], sizes, ws):
+                w.untyped_storage().resize_(n)
+                w.data.copy_(v)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, moved, dy), want))
+            del junk
