@@ -186,8 +186,13 @@ class GatedFFN:
         n = x.shape[0]
         if dy2.shape[0] != n:
             raise ValueError("dy must have the forward call's rows")
-        if x.shape[1] != self.H or pq.shape[2] != self.I:
+        if x.shape != (n, self.H) or h.shape != (n, self._pitch) or pq.shape != (2, n, self.I):
             raise ValueError("saved must be of a forward_train call of this block")
+        # (they may have been elsewhere in between: offloaded, or packed by a saved-tensor hook)
+        for t, dt in ((x, self.dtype), (h, self.dtype), (pq, torch.float32)):
+            if t.get_device() != self._index or t.dtype != dt or not (t is x or t.is_contiguous()):
+                raise ValueError(f"saved must be forward_train's tensors, on {self.device}: not {t.dtype} on {t.device}")
+        x = _rows(x, 8)
         H, I, new = self.H, self.I, self._new
         dx = new(dy.shape) if need[0] else None
         dwg = new((I, H)) if need[1] else None

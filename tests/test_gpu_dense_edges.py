@@ -145,3 +145,27 @@ def test_gated_ffn_reads_the_weights_that_were_saved(dev):
                 w.data.copy_(v)
             assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, moved, dy), want))
             del junk
+
+
+def test_ffn_saved_tensors_that_were_elsewhere(dev):
+    """What forward_train saved may be kept on the host meanwhile, and is refused unless it came back as it was."""
+    from glmx import GatedFFN, gated_ffn
+    x, wg, wu, wd, dy = block(dev, 40, 128, 72, HF, 431)
+    ffn = GatedFFN(wg, wu, wd)
+    _, saved = ffn.forward_train(x)
+    want = ffn.backward(dy, saved)
+    assert all(torch.equal(a, b) for a, b in zip(ffn.backward(dy, [t.cpu().to(dev) for t in saved]), want))
+    wide = torch.zeros(40, 140, device=dev, dtype=HF)
+    wide[:, 5:133] = x                                       # rows of another distance and alignment: laid out again
+    assert all(torch.equal(a, b) for a, b in zip(ffn.backward(dy, (wide[:, 5:133], *saved[1:])), want))
+    for i in range(3):
+        for bad in (saved[i].cpu(), saved[i].bfloat16(), saved[i][..., :-8], saved[i][:1]):
+            with pytest.raises(ValueError, match="saved|rows"):
+                ffn.backward(dy, [bad if j == i else t for j, t in enumerate(saved)])
+    with pytest.raises(ValueError, match="saved"):
+        ffn.backward(dy, (saved[0], saved[1].t().contiguous().t(), saved[2]))
+    leaf = wg.clone().requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
+        y = gated_ffn(x, leaf, wu, wd)
+    with pytest.raises(ValueError, match="cpu"):
+        y.backward(dy)
