@@ -35,7 +35,8 @@ struct Epi
     long long ldo;
     float* p; float* q;         // [M][N]
     float limit;
-    const void* x; const void* wg; const void* wu; long long ldx; int K;   // GATED with p: the operands, for the sums next to the limit
+    const void* x; const void* wg; const void* wu; long long ldx; int K;   // GATED with p: the operands, for the sums next to the limit,
+    const __nv_bfloat16* norms; // and their rows' norms, rounded up: [N] gate, [N] up, [M] tokens (NULL: every sum counts as next to it)
     const float* xs; const float* ws; const float* bias; // I8
 };
 
@@ -72,24 +73,88 @@ __device__ __forceinline__ void store_f32(float* d, const float (&v)[W])
     for (int i = 0; i < W / 4; ++i) reinterpret_cast<float4*>(d)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
 
-// sum_k x[t][k] w[n][k] in 64 bits by a warp (K a multiple of 8, both rows 16-byte aligned)
-static __device__ __noinline__ double warp_dot(const void* x, const void* w, int K, int bf16)
+// the two values of a 32-bit word, as a pair of fp32 registers
+template <bool BF16>
+__device__ __forceinline__ uint64_t unpack16(uint32_t w)
 {
+    float2 f;
+    if constexpr (BF16) f = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(f.x), "f"(f.y));
+    return r;
+}
+
+// Whether v = sum_k x[k] w[k], as silu(v) or |v|, is at most L in 64 bits; by a warp (K a multiple of 8, both rows 16-byte aligned). most: a bound
+// of |x| |w|. The sum is first formed in fp32, 256 chains of K / 256 fused products: it is within (K / 256 + 9) 2^-24 of the bound, and few of the
+// values that come here need the second one.
+template <bool BF16>
+static __device__ __noinline__ bool warp_within(const void* x, const void* w, int K, bool silu, float L, float most)
+{
+    const int k0 = (threadIdx.x & 31) * 8;
+    constexpr int U = 2;                                   // (more would have the kernel around spill)
+    // 2^-100: products that vanish
+    const float e = most * (float) (K / 256 + 12) * 0x1p-24f + 0x1p-100f;
+    if (e < 3e38f)
+    {
+        // two sets of U pieces of either row: one on its way while the other is added (volatile: fetched as written, not next to their use)
+        uint4 a[2][U], b[2][U];
+        uint64_t s[4] = {};
+        auto fetch = [&](int h, int k) {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+            {
+                a[h][j] = b[h][j] = make_uint4(0, 0, 0, 0);
+                if (k + 256 * j < K)
+                {
+                    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(a[h][j].x), "=r"(a[h][j].y), "=r"(a[h][j].z), "=r"(a[h][j].w) : "l"(static_cast<const uint16_t*>(x) + k + 256 * j));
+                    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(b[h][j].x), "=r"(b[h][j].y), "=r"(b[h][j].z), "=r"(b[h][j].w) : "l"(static_cast<const uint16_t*>(w) + k + 256 * j));
+                }
+            }
+        };
+        auto add = [&](int h) {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+            {
+                const uint32_t aw[4] = { a[h][j].x, a[h][j].y, a[h][j].z, a[h][j].w }, bw[4] = { b[h][j].x, b[h][j].y, b[h][j].z, b[h][j].w };
+#pragma unroll
+                for (int i = 0; i < 4; ++i) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(s[i]) : "l"(unpack16<BF16>(aw[i])), "l"(unpack16<BF16>(bw[i])));
+            }
+        };
+        fetch(0, k0);
+        for (int k = k0; k - k0 < K; k += 512 * U)
+        {
+            fetch(1, k + 256 * U);
+            add(0);
+            fetch(0, k + 512 * U);
+            add(1);
+        }
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v += __uint_as_float((uint32_t) s[i]) + __uint_as_float((uint32_t) (s[i] >> 32));
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        // (|silu'| < 1.1; the exponential and the division: some ulp)
+        const float y = silu ? v / (1.0f + expf(-v)) : fabsf(v), room = silu ? 1.1f * e + 0x1p-20f * L : e;
+        if (fabsf(y - L) > room) return y <= L;
+    }
     double d = 0.0;
-    for (int k = (threadIdx.x & 31) * 8; k < K; k += 256)
+    for (int k = k0; k < K; k += 256)
     {
         const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + k);
         const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d += (double) load16(&a, i, bf16) * (double) load16(&b, i, bf16);
+        for (int i = 0; i < 8; ++i) d += (double) load16(&a, i, BF16) * (double) load16(&b, i, BF16);
     }
     for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    return d;
+    return (silu ? d / (1.0 + exp(-d)) : fabs(d)) <= (double) L;
 }
 
 // h (and p, q) of 4 consecutive columns n .. n + 3 of token t, a multiple of 4; called by whole warps. acc, acc2: the sums of gate and up.
-// Which side of the limit a value falls on decides whether its gradient passes, and so must not hang on the last bits of
-// the tensor cores' truncated sums: within K 2^-25 (half a truncation for each MMA of 16 inputs, 16 times) the sum is formed again in 64 bits.
+// Which side of the limit a value falls on decides whether its gradient passes, and so must not hang on the last bits of the tensor cores'
+// truncated sums: within their error's bound the sum is formed again. An MMA of 16 inputs cuts each of its 17 addends to 2^-25 of
+// the largest one's power of two (measured: two bits below fp32's) and the sum to 2^-23: 5 2^-23 of the largest. The products' part in this is at
+// most |x| |w| (Cauchy-Schwarz) over all of K; the running sum v_k is at most |x_1..k| |w_1..k| and |v| + |x_k+1..| |w_k+1..|, hence
+// (|x| |w| + |v|) / 2 in each of the K / 16 steps, and less in a split's own sum. In all 5 2^-28 (K + 32) (|x| |w| + |v|); 96 for the splits' additions.
 __device__ __forceinline__ void emit_gated(const Epi& e, int t, int n, const uint32_t (&acc)[4], const uint32_t (&acc2)[4])
 {
     // N is a multiple of 8: all columns are inside, or none
@@ -97,8 +162,6 @@ __device__ __forceinline__ void emit_gated(const Epi& e, int t, int n, const uin
     const float L = e.limit;
     float g[4], u[4], s[4], act[4];
     bool kg[4], ku[4];
-    uint32_t near = 0;
-    const float win = L * ((float) e.K * 0x1p-25f + 0x1p-18f);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
@@ -108,11 +171,29 @@ __device__ __forceinline__ void emit_gated(const Epi& e, int t, int n, const uin
         act[i] = g[i] < -100.0f ? 0.0f : g[i] * s[i];      // silu(-inf) = 0 (not -inf * 0)
         kg[i] = L == 0.0f || act[i] <= L;
         ku[i] = L == 0.0f || fabsf(u[i]) <= L;
-        if (L != 0.0f) near |= (fabsf(act[i] - L) <= win ? 1u : 0u) << i | (fabsf(fabsf(u[i]) - L) <= win ? 16u : 0u) << i;
     }
     if (e.p && L != 0.0f)
     {
-        if (!in) near = 0;
+        uint32_t near = 0;
+        if (in)
+        {
+            const float inf = __int_as_float(0x7f800000);
+            float ng[4] = { inf, inf, inf, inf }, nu[4] = { inf, inf, inf, inf };
+            if (e.norms)
+            {
+                const uint2 a = *reinterpret_cast<const uint2*>(e.norms + n), b = *reinterpret_cast<const uint2*>(e.norms + e.N + n);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { ng[i] = load16(&a, i, 1); nu[i] = load16(&b, i, 1); }
+            }
+            const float nx = e.norms ? load16(e.norms, 2 * (size_t) e.N + t, 1) : 1.0f, c = (float) (e.K + 96) * 0x1.4p-26f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                // |silu'| < 1.1; 2^-18: the exponential and the division
+                const float wg = 1.1f * c * (nx * ng[i] + fabsf(g[i])) + L * 0x1p-18f, wu = c * (nx * nu[i] + fabsf(u[i]));
+                near |= (fabsf(act[i] - L) <= wg ? 1u : 0u) << i | (fabsf(fabsf(u[i]) - L) <= wu ? 16u : 0u) << i;
+            }
+        }
         uint32_t lanes = __ballot_sync(0xffffffffu, near != 0);
         while (lanes)
         {
@@ -124,9 +205,10 @@ __device__ __forceinline__ void emit_gated(const Epi& e, int t, int n, const uin
             {
                 const int b = __ffs(bits) - 1, c = nn + (b & 3);
                 bits &= bits - 1;
-                const double d = warp_dot(static_cast<const uint16_t*>(e.x) + (size_t) tt * e.ldx,
-                                          static_cast<const uint16_t*>(b < 4 ? e.wg : e.wu) + (size_t) c * e.K, e.K, e.bf16);
-                const bool keep = b < 4 ? d / (1.0 + exp(-d)) <= (double) L : fabs(d) <= (double) L;
+                const void* xr = static_cast<const uint16_t*>(e.x) + (size_t) tt * e.ldx;
+                const void* wr = static_cast<const uint16_t*>(b < 4 ? e.wg : e.wu) + (size_t) c * e.K;
+                const float bound = e.norms ? load16(e.norms, 2 * (size_t) e.N + tt, 1) * load16(e.norms, (size_t) (b < 4 ? 0 : e.N) + c, 1) : __int_as_float(0x7f800000);
+                const bool keep = e.bf16 ? warp_within<true>(xr, wr, e.K, b < 4, L, bound) : warp_within<false>(xr, wr, e.K, b < 4, L, bound);
                 if ((threadIdx.x & 31) == src)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -931,11 +1013,13 @@ __global__ void __launch_bounds__(COLS_THREADS, 2) cols_kernel(const __grid_cons
         constexpr int W = decltype(wide)::value;
         const int per = rows / W, units = ncols * per;
         const int u0 = (int) ((long long) units * split / splits), u1 = (int) ((long long) units * (split + 1) / splits);
+        // consecutive units in consecutive lanes; in different warps where a warp's units may have sums to form again, one after the other
+        const int place = EPI == EPI_GATED && a.e.p && a.e.limit != 0.0f ? lane * (COLS_THREADS / 32) + warp : tid;
         for (int ub = u0; ub < u1; ub += COLS_THREADS)
         {
             // (whole warps stay together: the last ones' lanes past the end work on the last unit and drop it)
-            const int u = min(ub + tid, u1 - 1);
-            const bool mine = ub + tid < u1;
+            const int u = min(ub + place, u1 - 1);
+            const bool mine = ub + place < u1;
             const int c = u / per, r = (u - c * per) * W;
             uint32_t v[W];
             auto sum = [&](uint32_t (&d)[W], uint32_t off) {

@@ -302,7 +302,9 @@ typedef struct
  * elements apart (a multiple of 8, at least H), y rows ldy apart (at least H). h: caller's scratch, ntok rows of
  * GLMX_FFN_PITCH(I) elements, 16-byte aligned; it holds the hidden rows afterwards. p, q: fp32 [ntok][I] or both NULL; with them the two factors of the backward pass are kept,
  *   p = min(silu(g), L) * [|u| <= L],  q = clamp(u, -L, L) * silu'(g) * [silu(g) <= L]
- * so that du = dh * p and dg = dh * q. */
+ * so that du = dh * p and dg = dh * q. Which side of L a sum is on is decided as in 64 bits. For that, a call with p, q and a limit keeps
+ * the operands' row norms in y until it writes y (where ldy = H, accumulate = 0, y is apart from x and holds 2 I + ntok 16-bit
+ * values; else, as in blocks of few tokens with I far above H, it forms every sum again, several times the time). */
 #define GLMX_FFN_PITCH(I) (((I) + 63) / 64 * 64)
 GLMX_API int glmx_ffn_forward(const glmx_ffn* ffn, const void* x, long long ldx, int ntok, void* y, long long ldy,
                               int y_dtype, int accumulate, void* h, float* p, float* q, void* stream);

@@ -169,3 +169,97 @@ def test_ffn_saved_tensors_that_were_elsewhere(dev):
         y = gated_ffn(x, leaf, wu, wd)
     with pytest.raises(ValueError, match="cpu"):
         y.backward(dy)
+
+
+def masks_are_exact(x, wg, wu, wd, limits):
+    """forward_train's factors are zero where the value in 64 bits is past the limit, and only there or where they are by themselves: a
+    sum's own error, at most 5 2^-28 (K + 96) (|x| |w| + |sum|), may make a value 0 that is not."""
+    from glmx import GatedFFN
+    xd, gd, ud = x.double(), wg.double(), wu.double()
+    g, u = xd @ gd.t(), xd @ ud.t()
+    act = g * torch.sigmoid(g)
+    err = lambda w, v: 5 * 2.0 ** -28 * (x.shape[1] + 96) * (xd.norm(dim=1)[:, None] * w.norm(dim=1)[None] + v.abs())
+    eg, eu = err(gd, g), err(ud, u)
+    for L in limits:
+        _, (_, _, pq) = GatedFFN(wg, wu, wd, act_limit=L).forward_train(x)
+        p, q = pq[0], pq[1]
+        inside, below = u.abs() <= L, act <= L
+        assert bool((p[~inside] == 0).all()) and bool((p[inside & (g.abs() > eg)] != 0).all()), L
+        # (silu' is at least 1/2 from g = 0 on)
+        assert bool((q[~below] == 0).all()) and bool((q[below & (g > eg) & (u.abs() > eu)] != 0).all()), L
+
+
+def near_values(x, wg, wu, lo, hi, n, seed):
+    """n limits that are the fp32 numbers next to values of the block between lo and hi"""
+    g, u = x.double() @ wg.double().t(), x.double() @ wu.double().t()
+    v = torch.cat([(g * torch.sigmoid(g)).flatten(), u.abs().flatten()])
+    v = v[(v > lo) & (v < hi)]
+    pick = torch.randint(0, v.numel(), (n,), generator=torch.Generator(device=x.device).manual_seed(seed), device=x.device)
+    return [float(torch.tensor(t, dtype=F32)) for t in v[pick].tolist()]
+
+
+# few and many rows, with and without room for the rows' norms in the output (2 I + T against T H values)
+@pytest.mark.parametrize("T,H,I", [(1, 64, 256), (3, 64, 2000), (5, 6144, 256), (70, 2048, 512), (700, 1032, 776), (900, 6144, 264)])
+def test_ffn_limit_far_below_the_sums(dev, T, H, I):
+    """The limit may be small beside the sums that are compared with it."""
+    x, wg, wu, wd, _ = block(dev, T, H, I, BF, 600 + T)
+    masks_are_exact(x, wg, wu, wd, near_values(x, wg, wu, 0.003, 0.03, 10, T))
+
+
+@pytest.mark.parametrize("dt", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,I", [(2, 64, 256), (6, 6144, 256), (40, 1160, 488), (700, 2048, 776)])
+def test_ffn_limit_with_cancelling_channels(dev, T, H, I, dt):
+    """Channels that cancel, at the row's ends: the sums between them are far larger than what is compared with the limit."""
+    x, wg, wu, wd, _ = block(dev, T, H, I, dt, 700 + T)
+    for k, v in ((0, 1.0), (1, 1.0), (H - 2, -1.0), (H - 1, -1.0)):
+        x[:, k] = v * 24
+        wg[:, k] = 8
+        wu[:, k] = 8
+    masks_are_exact(x, wg, wu, wd, near_values(x, wg, wu, 0.5, 3.0, 6, T) + near_values(x, wg, wu, 0.01, 0.1, 6, T + 1))
+
+
+def test_ffn_limit_with_an_output_that_cannot_hold_norms(dev):
+    """The output serves as scratch only where it is apart from the input, packed and not added to; its values are the same."""
+    import ctypes as C
+    from glmx import GatedFFN, _lib
+    T, H, I = 20, 512, 64
+    x, wg, wu, wd, _ = block(dev, T, H, I, BF, 801)
+    L = near_values(x, wg, wu, 0.01, 0.1, 1, 5)[0]
+    ffn = GatedFFN(wg, wu, wd, act_limit=L)
+    y, (_, h, pq) = ffn.forward_train(x)
+    st = torch.cuda.current_stream().cuda_stream
+
+    def call(xx, out, ldy, accumulate):
+        h2, pq2 = torch.empty_like(h), torch.empty_like(pq)
+        assert _lib.load().glmx_ffn_forward(C.byref(ffn._desc), xx.data_ptr(), xx.stride(0), T, out.data_ptr(), ldy, _lib.BF16, accumulate,
+                                            h2.data_ptr(), pq2[0].data_ptr(), pq2[1].data_ptr(), st) == _lib.OK
+        assert torch.equal(pq2, pq) and torch.equal(h2[:, :I], h[:, :I])
+    wide = torch.full((T, H + 8), 7.0, device=dev, dtype=BF)
+    call(x, wide, H + 8, 0)
+    assert torch.equal(wide[:, :H], y) and bool((wide[:, H:] == 7).all())
+    out = torch.zeros_like(y)
+    call(x, out, H, 1)
+    assert torch.equal(out, y)
+    same = x.clone()
+    call(same, same, H, 0)
+    assert torch.equal(same, y)
+    lap = torch.zeros(2 * T, H, device=dev, dtype=BF)        # the output begins in the middle of the input's rows
+    lap[:T] = x
+    call(lap[:T], lap[T // 2:T // 2 + T], H, 0)
+    assert torch.equal(lap[T // 2:T // 2 + T], y)
+
+
+def test_ffn_limit_with_rows_of_zeros_infinities_and_nan(dev):
+    """Rows whose norm is 0, infinite or NaN leave the others as they are."""
+    from glmx import GatedFFN
+    for T in (6, 300):
+        x, wg, wu, wd, dy = block(dev, T, 512, 136, BF, 811)
+        ffn = GatedFFN(wg, wu, wd, act_limit=0.75)
+        y, (_, h, pq) = ffn.forward_train(x)
+        x[1], x[3, 5], x[4, 7], x[5, 2] = 0, math.inf, math.nan, 3e38
+        y2, (_, h2, pq2) = ffn.forward_train(x)
+        keep = [i for i in range(T) if i not in (1, 3, 4, 5)]
+        assert torch.equal(y2[keep], y[keep]) and torch.equal(pq2[:, keep], pq[:, keep])
+        assert bool((y2[1] == 0).all()) and bool((pq2[:, 1] == 0).all()) and bool(y2[4].isnan().all())
+        u = (x[5:6].double() @ wu.double().t())[0]
+        assert torch.equal(pq2[0, 5] == 0, (u.abs() > 0.75) | (pq2[0, 5] == 0)) and bool(torch.isfinite(y2[5]).all())
