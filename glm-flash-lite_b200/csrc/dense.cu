@@ -23,30 +23,19 @@ int dense_device()
 
 cudaError_t dense_err_ptr(int** p)
 {
-    static int* ptr[64] = {};
-    const int d = dense_device();
-    if (d < 0 || d >= 64) return cudaErrorInvalidDevice;
-    if (!ptr[d])
-    {
-        int* q = nullptr;
-        const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&q), g_dense_err);
-        if (e != cudaSuccess) return e;
-        ptr[d] = q;
-    }
-    *p = ptr[d];
-    return cudaSuccess;
+    static PerDevice<int*> ptr;
+    int* const* v;
+    const cudaError_t e = ptr.get(dense_device(), &v, [](int*& q) { return cudaGetSymbolAddress(reinterpret_cast<void**>(&q), g_dense_err); });
+    if (e == cudaSuccess) *p = *v;
+    return e;
 }
 
 int dense_sms(int device)
 {
-    static int n[64] = {};
-    if (!n[device])
-    {
-        int v = 0;
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || v < 2) v = 2;
-        n[device] = v;
-    }
-    return n[device];
+    static PerDevice<int> sms;
+    const int* n;
+    const cudaError_t e = sms.get(device, &n, [&](int& v) { return cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device); });
+    return e == cudaSuccess && *n >= 2 ? *n : 2;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -55,15 +44,13 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 
 cudaError_t dense_map(CUtensorMap* m, int dtype, const Mat& t, int box_inner, int box_rows)
 {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn)
-    {
+    static const EncodeTiledFn fn = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        if (!fn) return cudaErrorNotSupported;
-    }
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+    }();
+    if (!fn) return cudaErrorNotSupported;
     const int size = dtype == GLMX_F32 ? 4 : dtype == GLMX_F16 || dtype == GLMX_BF16 ? 2 : 1;
     const cuuint64_t dims[2] = { (cuuint64_t) t.inner, (cuuint64_t) t.rows };
     const cuuint64_t strides[1] = { (cuuint64_t) t.pitch * size };

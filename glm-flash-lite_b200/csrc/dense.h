@@ -5,6 +5,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
+
 #include "glmx.h"
 #include "glmx_internal.h"
 
@@ -23,6 +26,44 @@ inline int dense_cuda_fail(cudaError_t e, const char* what)
 }
 
 inline bool dense_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What is found out once a device. Threads whose first calls meet: one runs fill(value), the others wait for it; a value is seen whole or
+// not at all. After an error the next call tries again.
+template <typename T>
+class PerDevice
+{
+    std::mutex m;
+    std::atomic<bool> ready[64] = {};
+    T value[64] = {};
+
+public:
+    template <typename F>
+    cudaError_t get(int device, const T** out, F fill)
+    {
+        if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+        if (!ready[device].load(std::memory_order_acquire))
+        {
+            std::lock_guard<std::mutex> lock(m);
+            if (!ready[device].load(std::memory_order_relaxed))
+            {
+                T v{};
+                const cudaError_t e = fill(v);
+                if (e != cudaSuccess) return e;
+                value[device] = v;
+                ready[device].store(true, std::memory_order_release);
+            }
+        }
+        *out = &value[device];
+        return cudaSuccess;
+    }
+};
+
+// the dynamic shared memory that a kernel's launches may ask for, set once
+inline cudaError_t dense_smem(PerDevice<int>& set, int device, const void* kernel, int bytes)
+{
+    const int* done;
+    return set.get(device, &done, [&](int&) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+}
 
 int dense_device();                          // the current device, or -1
 int dense_sms(int device);

@@ -1090,14 +1090,9 @@ cudaError_t launch_pair(int dtype, int nprob, const Product* pr, int nseg, int K
 {
     auto kernel = pair_kernel<I8, A_MN, B_MN, EPI>;
     const int dev = dense_device();
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    static bool ready[64] = {};
-    cudaError_t err;
-    if (!ready[dev])
-    {
-        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM - 1024)) != cudaSuccess) return err;
-        ready[dev] = true;
-    }
+    static PerDevice<int> smem;
+    cudaError_t err = dense_smem(smem, dev, reinterpret_cast<const void*>(kernel), PAIR_SMEM - 1024);
+    if (err != cudaSuccess) return err;
     PairMaps maps;
     PairArgs a{};
     a.nprob = nprob; a.nseg = nseg; a.K = K; a.bk = I8 ? 128 : 64; a.BN = BN;
@@ -1215,36 +1210,30 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, const ColsCapacity& 
 template <bool I8, bool W_MN, int EPI>
 cudaError_t cols_capacity(int dev, const ColsCapacity** out)
 {
-    auto kernel = cols_kernel<I8, W_MN, EPI>;
-    static ColsCapacity cap[64] = {};
-    static bool ready[64] = {};
-    if (!ready[dev])
-    {
+    static PerDevice<ColsCapacity> capacity;
+    return capacity.get(dev, out, [](ColsCapacity& cap) {
+        auto kernel = cols_kernel<I8, W_MN, EPI>;
         cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, COLS_SMEM1);
         if (err == cudaSuccess)
             err = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        for (int i = 0; i < 2; ++i)
-            for (int s = 1; s <= 8 && err == cudaSuccess; ++s)
-            {
-                cudaLaunchConfig_t cfg = {};
-                cfg.gridDim = dim3(s, 1024);
-                cfg.blockDim = dim3(COLS_THREADS);
-                cfg.dynamicSmemBytes = COLS_SMEM1;
-                cudaLaunchAttribute attr[1];
-                attr[0].id = cudaLaunchAttributeClusterDimension;
-                attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-                cfg.attrs = attr;
-                cfg.numAttrs = 1;
-                err = cudaOccupancyMaxActiveClusters(&cap[dev].n[i][s], kernel, &cfg);
-                // the occupancy calculator counts one CTA an SM for every kernel that allocates tensor memory; two of the smaller kind do
-                // run at once (seen by their clocks and SM numbers)
-                if (i == 0) cap[dev].n[i][s] *= 2;
-            }
-        if (err != cudaSuccess) return err;
-        ready[dev] = true;
-    }
-    *out = &cap[dev];
-    return cudaSuccess;
+        for (int s = 1; s <= 8 && err == cudaSuccess; ++s)
+        {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(s, 1024);
+            cfg.blockDim = dim3(COLS_THREADS);
+            cfg.dynamicSmemBytes = COLS_SMEM1;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            err = cudaOccupancyMaxActiveClusters(&cap.n[1][s], kernel, &cfg);
+            // the occupancy calculator counts one CTA an SM for every kernel that allocates tensor memory; two of the smaller kind do
+            // run at once (seen by their clocks and SM numbers)
+            cap.n[0][s] = 2 * cap.n[1][s];
+        }
+        return err;
+    });
 }
 
 template <bool I8, bool W_MN, int EPI>
@@ -1285,7 +1274,6 @@ template <bool I8, bool W_MN, int EPI>
 cudaError_t launch_product(int dtype, const Product& pr, int nseg, int K, bool prefetch, cudaStream_t st)
 {
     const int dev = dense_device();
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     const int nk = nseg * ((K + (I8 ? 127 : 63)) / (I8 ? 128 : 64)), sms = dense_sms(dev);
     const ColsCapacity* cap;
     const cudaError_t err = cols_capacity<I8, W_MN, EPI>(dev, &cap);

@@ -804,13 +804,8 @@ cudaError_t launch_sample(const SampleArgs& a0, int B, cudaStream_t st)
     int dev = -1;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
-    if (dev >= 64) return cudaErrorInvalidDevice;
-    static bool ready[64] = {};
-    if (!ready[dev])
-    {
-        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SLICE_MAX * 4 + 64)) != cudaSuccess) return err;
-        ready[dev] = true;
-    }
+    static PerDevice<int> smem;
+    if ((err = dense_smem(smem, dev, reinterpret_cast<const void*>(kernel), SLICE_MAX * 4 + 64)) != cudaSuccess) return err;
     SampleArgs a = a0;
     // CTAs per row: all 8 from 16384 logits on; a slice below 2048 logits would wait more than it works
     int nc = 1;

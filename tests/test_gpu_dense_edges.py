@@ -263,3 +263,56 @@ def test_ffn_limit_with_rows_of_zeros_infinities_and_nan(dev):
         assert bool((y2[1] == 0).all()) and bool((pq2[:, 1] == 0).all()) and bool(y2[4].isnan().all())
         u = (x[5:6].double() @ wu.double().t())[0]
         assert torch.equal(pq2[0, 5] == 0, (u.abs() > 0.75) | (pq2[0, 5] == 0)) and bool(torch.isfinite(y2[5]).all())
+
+
+# ---- first calls -------------------------------------------------------------------------------------------------------
+
+def test_first_calls_of_several_threads_at_once():
+    """A process whose threads make their first calls together gives the bits of one that makes them one after the other."""
+    import subprocess
+    import sys
+    from conftest import PKG
+    code = """
+import hashlib, sys, threading, torch
+sys.path.insert(0, %r)
+import glmx
+d, together = 'cuda', sys.argv[1] == 'together'
+g = torch.Generator(device=d).manual_seed(1)
+rn = lambda *s: torch.randn(*s, generator=g, device=d)
+w, wd, dy = (rn(776, 1024) / 32).bfloat16(), (rn(1024, 776) / 28).bfloat16(), rn(40, 1024).bfloat16()
+xs = [rn(n, 1024).bfloat16() for n in (1, 7, 40, 40, 200, 7, 1, 200)]
+u = torch.rand(200, generator=g, device=d)
+wq, ws = torch.randint(-99, 99, (776, 1024), device=d, dtype=torch.int8, generator=g), torch.rand(776, device=d, generator=g)
+ffn, lin = glmx.GatedFFN(w, w, wd), glmx.Int8Linear(wq, ws)
+torch.cuda.synchronize()
+out, start = [None] * len(xs), threading.Barrier(len(xs))
+def run(i):
+    torch.cuda.set_device(0)
+    if together:
+        start.wait()
+    x = xs[i]
+    with torch.cuda.stream(torch.cuda.Stream()):
+        y, saved = ffn.forward_train(x)
+        r = (y, *ffn.backward(x, saved), lin(x), glmx.sample(y, u[:len(x)], top_p=0.9))
+        torch.cuda.current_stream().synchronize()
+    out[i] = r
+threads = [threading.Thread(target=run, args=(i,)) for i in range(len(xs))]
+for t in threads:
+    t.start()
+    if not together:
+        t.join()
+for t in threads:
+    t.join()
+glmx.dense_check()
+h = hashlib.sha256()
+for r in out:
+    for t in r:
+        h.update(t.float().cpu().numpy().tobytes())
+print('digest', h.hexdigest())
+""" % PKG
+    digest = []
+    for how in ("one by one", "together", "together", "together"):
+        r = subprocess.run([sys.executable, "-c", code, how], capture_output=True, text=True, timeout=240)
+        assert r.returncode == 0 and "digest" in r.stdout, r.stderr[-2000:]
+        digest.append(r.stdout.split("digest")[1].strip())
+    assert len(set(digest)) == 1
