@@ -538,6 +538,12 @@ __device__ __forceinline__ void copy_rows(const Epi& e, const uint4* stg, int ro
     }
 }
 
+// Shared memory of a CTA that allocates `cols` columns of tensor memory: at least the same share of the SM's, so that CTAs which fit
+// an SM together, of whatever launches and streams, never want more than its 512 columns. Allocation waits for columns without limit, and CTAs
+// of a cluster wait for one another: two clusters that each held columns that the other's CTAs wait for would hang.
+constexpr int tmem_smem(int cols, int bytes) { return bytes > cols * 452 ? bytes : cols * 452; }
+static_assert((512 + 32) * 452 > 228 * 1024, "one allocation more than 512 columns does not fit an SM's 228 KB");
+
 // ---- pair_kernel -------------------------------------------------------------------------------------------------------
 
 constexpr int MAXPROB = 3;
@@ -572,7 +578,8 @@ constexpr int pair_stages(int bn)
     const int n = (PAIR_SMEM - 1024 - 1024 - PAIR_STG) / pair_stage(bn);   // 1 KB of static shared memory, 1 KB of alignment
     return n > PAIR_STAGES_MAX ? PAIR_STAGES_MAX : n;
 }
-constexpr int pair_smem(int bn) { return 1024 + pair_stages(bn) * pair_stage(bn) + PAIR_STG; }
+constexpr int pair_smem(int bn) { return tmem_smem(512, 1024 + pair_stages(bn) * pair_stage(bn) + PAIR_STG); }
+static_assert(pair_smem(64) <= PAIR_SMEM - 1024 && pair_smem(128) <= PAIR_SMEM - 1024 && pair_smem(192) <= PAIR_SMEM - 1024 && pair_smem(256) <= PAIR_SMEM - 1024, "");
 
 // I8: signed bytes; A_MN / B_MN: operand stored [K][rows]; EPI
 template <bool I8, bool A_MN, bool B_MN, int EPI>
@@ -1207,6 +1214,15 @@ inline ColsPlan cols_plan(int M, int N, bool gated, int nk, const ColsCapacity& 
     return p;
 }
 
+inline int cols_tmem(const ColsPlan& p)
+{
+    int n = 32;
+    while (n < p.NT) n *= 2;
+    return n;
+}
+
+inline int cols_smem(const ColsPlan& p) { return tmem_smem(cols_tmem(p), 1024 + p.stages * (16384 + p.NT * 128)); }
+
 template <bool I8, bool W_MN, int EPI>
 cudaError_t cols_capacity(int dev, const ColsCapacity** out)
 {
@@ -1245,8 +1261,7 @@ cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, const Col
     ColsArgs a{};
     a.nseg = nseg; a.K = K; a.bk = I8 ? 128 : 64;
     a.NT = p.NT; a.xrows = pr.e.M < p.NT ? pr.e.M : p.NT; a.stages = p.stages; a.mtiles = p.mtiles; a.prefetch = prefetch;
-    a.tcols = 32;
-    while (a.tcols < p.NT) a.tcols *= 2;
+    a.tcols = cols_tmem(p);
     a.idesc = tc_idesc(I8, dtype == GLMX_BF16, W_MN, false, 128, p.NT);
     if ((err = dense_err_ptr(&a.err)) != cudaSuccess) return err;
     a.e = pr.e;
@@ -1257,7 +1272,7 @@ cudaError_t launch_cols(int dtype, const Product& pr, int nseg, int K, const Col
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.mtiles * p.ttiles);
     cfg.blockDim = dim3(COLS_THREADS);
-    cfg.dynamicSmemBytes = 1024 + (size_t) p.stages * (16384 + p.NT * 128);
+    cfg.dynamicSmemBytes = cols_smem(p);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
