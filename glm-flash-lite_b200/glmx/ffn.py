@@ -16,8 +16,10 @@ from . import _lib
 from ._lib import check
 from .layer import _dt
 
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream's handle, without a Stream object around it
+# the current device, and the current stream's handle without a Stream object around it; by the public way where a torch (one without
+# CUDA, say) has not got these
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: int(torch.cuda.current_stream(index).cuda_stream))
 
 
 def _on(index: int, stream):
