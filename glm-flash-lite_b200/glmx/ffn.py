@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._lib import check
@@ -50,6 +51,11 @@ def _rows(t: torch.Tensor, align: int, pitch_of_copy: int = 64) -> torch.Tensor:
     else:
         c.copy_(t)
     return c
+
+
+def _no_tangent(t: torch.Tensor) -> None:
+    if unpack_dual(t).tangent is not None:
+        raise RuntimeError("the gated feed-forward block has no forward-mode derivative")
 
 
 def dense_check(device=None, stream=None) -> None:
@@ -110,6 +116,7 @@ class GatedFFN:
         return f
 
     def _pack(self, w: torch.Tensor) -> torch.Tensor:
+        _no_tangent(w)
         if w.is_contiguous() and w.data_ptr() % 16 == 0:
             return w
         with torch.cuda.device(self._index):
@@ -122,7 +129,13 @@ class GatedFFN:
             raise TypeError(f"{what} must be {self.dtype}, not {x.dtype}")
         if x.get_device() != self._index:
             raise ValueError(f"{what} on {x.device}, weights on {self.device}")
+        _no_tangent(x)
         return _rows(x if x.dim() == 2 else x.reshape(-1, self.H), 8)
+
+    @staticmethod
+    def _no_gradient(x, out) -> None:
+        if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+            raise RuntimeError("GatedFFN.forward gives no gradient to x or out, which require one: use gated_ffn, or torch.no_grad()")
 
     def _new(self, shape, dtype=None):
         return self.w_gate.new_empty(shape) if dtype is None else self.w_gate.new_empty(shape, dtype=dtype)
@@ -137,7 +150,8 @@ class GatedFFN:
                 stream=None) -> torch.Tensor:
         """y [..., H] for x [..., H] of the block's dtype. out_dtype: the block's dtype (default) or fp32; out: a
         contiguous tensor of x's shape to write instead, accumulate=True to add to it (a shared expert's output onto
-        MoELayer.forward's)."""
+        MoELayer.forward's). No gradient: where x or out requires one, the call is refused (gated_ffn is differentiable)."""
+        self._no_gradient(x, out)
         ctx = _on(self._index, stream)
         if ctx is not None:
             with ctx:

@@ -152,8 +152,10 @@ class MoELayer:
         workspace: a uint8 CUDA tensor of at least workspace_bytes(ntok, topk) to use instead of the layer's own (calls
         that may run at the same time on different streams need workspaces of their own).
         dense_shared: a GatedFFN (an unquantised shared expert over the same H) whose output for x, rounded to its dtype, is
-        added to out; out must be fp32 or of its dtype, and share no memory with x."""
+        added to out; out must be fp32 or of its dtype, and share no memory with x. As GatedFFN.forward, it gives no gradient, and is
+        refused where x or out requires one."""
         if dense_shared is not None:
+            dense_shared._no_gradient(x, out)
             if dense_shared.H != self.H or dense_shared.device != self.device:
                 raise ValueError("dense_shared must have the layer's hidden size and device")
             if (out_dtype if out is None else out.dtype) not in (torch.float32, dense_shared.dtype):

@@ -316,3 +316,38 @@ print('digest', h.hexdigest())
         assert r.returncode == 0 and "digest" in r.stdout, r.stderr[-2000:]
         digest.append(r.stdout.split("digest")[1].strip())
     assert len(set(digest)) == 1
+
+
+# ---- gradients that a call does not give -------------------------------------------------------------------------------
+
+def test_ffn_refuses_to_drop_a_gradient(dev):
+    """The inference calls refuse tensors that require a gradient, unless gradients are off; nothing is written then."""
+    from glmx import GatedFFN, MoELayer, gated_ffn, synth
+    x, wg, wu, wd, _ = block(dev, 4, 512, 96, HF, 901)
+    ffn = GatedFFN(wg.requires_grad_(True), wu, wd)          # (the weights of a block are constants of its calls)
+    want = ffn(x)
+    assert not want.requires_grad
+    leaf, out = x.clone().requires_grad_(True), torch.zeros_like(x).requires_grad_(True)
+    layer = MoELayer.from_bank(synth.make_bank(512, 256, 8, shared=False, seed=3), device=dev)
+    sel, w = torch.tensor([[0, 1]] * 4, dtype=torch.int32, device=dev), torch.full((4, 2), 0.5, device=dev)
+    held = torch.zeros(4, 512, device=dev)
+    for call in (lambda: ffn(leaf), lambda: ffn(leaf * 2), lambda: ffn(x, out=out), lambda: ffn(x, out=out, accumulate=True),
+                 lambda: ffn(leaf, stream=torch.cuda.current_stream()), lambda: layer.forward(leaf, sel, w, out=held, dense_shared=ffn)):
+        with pytest.raises(RuntimeError, match="gated_ffn"):
+            call()
+    assert float(out.detach().abs().max()) == 0 and float(held.abs().max()) == 0
+    with torch.no_grad():
+        assert torch.equal(ffn(leaf), want) and torch.equal(ffn(x, out=out), want)
+        assert torch.equal(layer.forward(leaf, sel, w, dense_shared=ffn), layer.forward(x, sel, w, dense_shared=ffn))
+    assert torch.equal(ffn(leaf.detach()), want)
+    # leading tangents are refused with gradients on and off
+    import torch.autograd.forward_ad as fw
+    for on in (False, True):
+        with torch.set_grad_enabled(on), fw.dual_level():
+            dual = fw.make_dual(x, torch.ones_like(x))
+            dual_w = fw.make_dual(wu, torch.ones_like(wu))
+            for call in (lambda: gated_ffn(dual, wg, wu, wd), lambda: gated_ffn(x, wg, dual_w, wd), lambda: ffn(dual),
+                         lambda: ffn.forward_train(dual), lambda: GatedFFN(wg, dual_w, wd)):
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    call()
+    assert torch.equal(ffn(x), want)
