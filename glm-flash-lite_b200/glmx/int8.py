@@ -7,6 +7,8 @@ the head.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -68,10 +70,16 @@ def _collapses(t: torch.Tensor) -> bool:
     return all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2))
 
 
-def _vec(t: torch.Tensor, n: int, what: str, device) -> torch.Tensor:
-    if t.dtype != torch.float32 or t.numel() != n or t.get_device() != device.index:
-        raise ValueError(f"{what} must be fp32 with {n} elements on {device}")
+def _vec(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
+    """t, fp32 with an element for each of `shape`, in its order: of that shape but for dimensions of size 1, or either of them flat"""
+    if t.dtype != torch.float32 or t.get_device() != device.index or not (
+            t.shape == shape or (t.numel() == math.prod(shape) and (len(shape) < 2 or t.dim() == 1 or _long(t.shape) == _long(shape)))):
+        raise ValueError(f"{what} must be fp32 {list(shape)} on {device}, not {t.dtype} {list(t.shape)} on {t.device}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _long(shape) -> list:
+    return [n for n in shape if n != 1]
 
 
 class Int8Linear:
@@ -93,8 +101,8 @@ class Int8Linear:
         self._index = wq.get_device()
         with torch.cuda.device(self._index):
             self.wq = _rows(wq, 16, _PITCH)
-            self.w_scale = _vec(w_scale, self.N, "w_scale", self.device)
-            self.bias = None if bias is None else _vec(bias, self.N, "bias", self.device)
+            self.w_scale = _vec(w_scale, (self.N,), "w_scale", self.device)
+            self.bias = None if bias is None else _vec(bias, (self.N,), "bias", self.device)
         self._w, self._ldw, self._ws = self.wq.data_ptr(), self.wq.stride(0), self.w_scale.data_ptr()
         self._bias = 0 if bias is None else self.bias.data_ptr()
 
@@ -107,7 +115,7 @@ class Int8Linear:
     def matmul(self, xq: torch.Tensor, x_scale: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None,
                stream=None) -> torch.Tensor:
         """y [..., N] from quantised rows xq int8 [..., K] and x_scale fp32 [...] (quantize_rows' results: one
-        quantisation serves several linears)."""
+        quantisation serves several linears; a flat x_scale has the rows' order)."""
         if xq.get_device() != self._index:
             raise ValueError(f"xq on {xq.device}, weights on {self.device}")
         ctx = _on(self._index, stream)
@@ -116,7 +124,7 @@ class Int8Linear:
                 return self.matmul(xq, x_scale, out, out_dtype)
         x2 = _q_rows(xq, "xq", self.K)
         T = x2.shape[0]
-        xs = _vec(x_scale, T, "x_scale", self.device)
+        xs = _vec(x_scale, xq.shape[:-1], "x_scale", self.device)
         if out is None:
             dt = out_dtype or self.out_dtype or torch.bfloat16
             if dt not in _FLOAT:

@@ -351,3 +351,34 @@ def test_ffn_refuses_to_drop_a_gradient(dev):
                 with pytest.raises((RuntimeError, NotImplementedError)):
                     call()
     assert torch.equal(ffn(x), want)
+
+
+# ---- 8-bit linears -----------------------------------------------------------------------------------------------------
+
+def test_int8_scales_have_the_rows_shape(dev):
+    """A scale for each row: of the rows' leading shape, with or without dimensions of size 1, or flat in the rows' order."""
+    from glmx import Int8Linear, quantize_rows
+    gen = torch.Generator(device=dev).manual_seed(911)
+    x, w = torch.randn(2, 3, 64, generator=gen, device=dev), torch.randn(24, 64, generator=gen, device=dev)
+    lin = Int8Linear.from_weight(w, out_dtype=F32)
+    want = lin(x)
+    q, s = quantize_rows(x)
+    for t in (s, s.reshape(6), s[..., None], s[None], s.t().contiguous().t()):
+        assert torch.equal(lin.matmul(q, t), want)
+    assert torch.equal(lin.matmul(q.transpose(0, 1), s.t()), want.transpose(0, 1))
+    assert torch.equal(lin.matmul(q.reshape(6, 64), s), want.view(6, 24))
+    for t in (s.t(), s.t().contiguous(), s.reshape(6, 1).expand(6, 2), s[:1], s[:, :2], s.double(), s.cpu(), s.reshape(1, 6, 1).expand(2, 6, 1)):
+        with pytest.raises(ValueError, match="x_scale"):
+            lin.matmul(q, t)
+    one = lin(x[0, :1])
+    q, s = quantize_rows(x[0, :1])
+    for t in (s, s[0], s.reshape(1, 1, 1)):
+        assert torch.equal(lin.matmul(q, t), one)
+    assert torch.equal(lin.matmul(q[0], s[0]), one[0]) and torch.equal(lin.matmul(q[0], s), one[0])
+    assert lin.matmul(q[:0], s[:0]).shape == (0, 24)
+    b = torch.randn(24, generator=gen, device=dev)
+    want = Int8Linear(lin.wq, lin.w_scale, b)(x)
+    assert torch.equal(Int8Linear(lin.wq, lin.w_scale[:, None], b[None])(x), want)
+    for bad in (dict(bias=b[:23]), dict(w_scale=lin.w_scale[:1]), dict(w_scale=lin.w_scale.half()), dict(bias=b.cpu())):
+        with pytest.raises(ValueError, match="must be fp32"):
+            Int8Linear(**(dict(wq=lin.wq, w_scale=lin.w_scale, bias=b) | bad))
