@@ -1,10 +1,12 @@
-// What the dense operators' launches share: tensor maps, device facts, and the error word (glmx_dense_check): one per device,
-// sticky, set by a kernel whose bounded wait expired.
+// What the dense operators' launches share: tensor maps, device facts, and the error word (glmx_dense_check): one per device, for the
+// kernels of all streams; sticky, set by a kernel whose bounded wait expired.
 #include "gemm_tc.cuh"
 
 namespace glmx {
 
 static __device__ int g_dense_err;
+
+static __global__ void clear_kernel(int* p, int bits) { atomicAnd(p, ~bits); }
 
 int dense_device()
 {
@@ -74,8 +76,14 @@ extern "C" int glmx_dense_check(void* stream, int* flags)
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = dense_err_ptr(&p);
     if (e == cudaSuccess) e = cudaMemcpyAsync(&v, p, sizeof(int), cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && v)
+    {
+        // the bits that are reported, no others: a kernel of another stream may have set one since
+        clear_kernel<<<1, 1, 0, st>>>(p, v);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    }
     if (e != cudaSuccess) return dense_cuda_fail(e, "glmx_dense_check");
     if (flags) *flags = v;
     return v ? dense_fail(GLMX_E_DEVICE, "glmx_dense_check: a bounded wait expired in a dense operator") : GLMX_OK;

@@ -59,8 +59,8 @@ def _no_tangent(t: torch.Tensor) -> None:
 
 
 def dense_check(device=None, stream=None) -> None:
-    """Synchronises the stream and raises GlmxError where a dense operator on the device gave up a bounded wait since the
-    last check (glmx_dense_check)."""
+    """Synchronises the stream and raises GlmxError where a dense operator on the device, on whichever stream, gave up a bounded
+    wait since the last check (glmx_dense_check)."""
     index = torch.device("cuda" if device is None else device).index
     with torch.cuda.device(_current_device() if index is None else index):
         s = stream if stream is not None else torch.cuda.current_stream()

@@ -348,7 +348,8 @@ GLMX_API int glmx_sample(const void* logits, int dtype, long long ld, int B, int
                          const float* min_p, float min_p0, void* ids, int ids_dtype, void* stream);
 
 /* Synchronises `stream` and reads the dense operators' device error word on the current device (a bounded wait that expired):
- * GLMX_OK or GLMX_E_DEVICE; *flags receives the bits. The word is sticky; the call clears it. */
+ * GLMX_OK or GLMX_E_DEVICE; *flags receives the bits. There is one word for the kernels of all streams of the device, whoever launched them: what
+ * other streams have in flight may still set it. A bit stays set until a call has reported it; that call clears it. */
 GLMX_API int glmx_dense_check(void* stream, int* flags);
 
 #ifdef __cplusplus

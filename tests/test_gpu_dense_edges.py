@@ -382,3 +382,63 @@ def test_int8_scales_have_the_rows_shape(dev):
     for bad in (dict(bias=b[:23]), dict(w_scale=lin.w_scale[:1]), dict(w_scale=lin.w_scale.half()), dict(bias=b.cpu())):
         with pytest.raises(ValueError, match="must be fp32"):
             Int8Linear(**(dict(wq=lin.wq, w_scale=lin.w_scale, bias=b) | bad))
+
+
+# ---- the error word ----------------------------------------------------------------------------------------------------
+
+CHECK_PROGRAM = r"""
+#include "dense.cu"
+#include <cstdio>
+#include <thread>
+namespace glmx { void set_error(const std::string&) {} }
+
+static __global__ void or_kernel(int* p, int bits, int pause)
+{
+    for (int i = 0; i < pause; ++i) __nanosleep(100);
+    atomicOr(p, bits);
+}
+
+int main()
+{
+    int* p = nullptr;
+    cudaStream_t a, b;
+    if (cudaStreamCreateWithFlags(&a, cudaStreamNonBlocking) || cudaStreamCreateWithFlags(&b, cudaStreamNonBlocking) || glmx::dense_err_ptr(&p)) return 1;
+    int flags = -1, lost = 0, errors = 0;
+    errors += glmx_dense_check(a, &flags) != GLMX_OK || flags != 0;
+    or_kernel<<<1, 1, 0, a>>>(p, 5, 0);
+    errors += glmx_dense_check(a, &flags) != GLMX_E_DEVICE || flags != 5;
+    errors += glmx_dense_check(a, nullptr) != GLMX_OK;
+    // one error is known when the check begins; another one comes from the other stream at some time during it
+    for (int i = 0; i < 3000; ++i)
+    {
+        const int late = 1 << (1 + i % 30);
+        or_kernel<<<1, 1, 0, a>>>(p, 1, 0);
+        std::thread other([&] { or_kernel<<<1, 1, 0, b>>>(p, late, i / 30 % 100); });
+        int first = 0, second = 0;
+        glmx_dense_check(a, &first);
+        other.join();
+        cudaStreamSynchronize(b);
+        glmx_dense_check(a, &second);
+        lost += ((first | second) & late) == 0 || (first & 1) == 0;
+    }
+    std::printf("errors %d lost %d %s\n", errors, lost, cudaGetErrorString(cudaDeviceSynchronize()));
+    return 0;
+}
+"""
+
+
+def test_dense_check_loses_no_error(tmp_path):
+    """An error of another stream that comes while a check runs is reported by that check or by the next one."""
+    import os
+    import shutil
+    import subprocess
+    from conftest import PKG, REPO
+    nvcc = os.environ.get("NVCC") or shutil.which("nvcc")
+    if not nvcc:
+        pytest.skip("no nvcc")
+    src, exe = tmp_path / "check.cu", tmp_path / "check"
+    src.write_text(CHECK_PROGRAM)
+    subprocess.run([nvcc, "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a", "--expt-relaxed-constexpr",
+                    "-I" + os.path.join(REPO, "include"), "-I" + os.path.join(PKG, "csrc"), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=120).stdout
+    assert out.split() == ["errors", "0", "lost", "0", "no", "error"]
