@@ -62,7 +62,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     if not isinstance(top_k, torch.Tensor):
         top_k = max(0, min(int(top_k), V))
     elif top_k.dtype != torch.int32:
-        top_k = top_k.clamp(0, V)                # before the conversion: a larger number keeps its meaning
+        # limited before the conversion, where a larger number keeps its meaning (V itself may be beyond 8 and 16 bits)
+        top_k = (top_k if top_k.is_floating_point() else top_k.long()).clamp(0, V)
     k, kp, k0 = _param(top_k, torch.int32, B, index, "top_k")
     p, pp, p0 = _param(top_p, torch.float32, B, index, "top_p")
     m, mp, m0 = _param(min_p, torch.float32, B, index, "min_p")

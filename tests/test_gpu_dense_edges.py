@@ -442,3 +442,15 @@ def test_dense_check_loses_no_error(tmp_path):
                     "-I" + os.path.join(REPO, "include"), "-I" + os.path.join(PKG, "csrc"), str(src), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=120).stdout
     assert out.split() == ["errors", "0", "lost", "0", "no", "error"]
+
+
+@pytest.mark.parametrize("kt", [torch.uint8, torch.int8, torch.int16, torch.int64, torch.float32, torch.float16])
+def test_sample_top_k_of_any_type(dev, kt):
+    """top_k in any number type, also one that cannot hold the vocabulary's size."""
+    from glmx import sample
+    gen = torch.Generator(device=dev).manual_seed(921)
+    logits, u = torch.randn(5, 70001, generator=gen, device=dev) * 3, torch.rand(5, generator=gen, device=dev)
+    k = torch.tensor([0, 1, 5, 100, 127], device=dev)
+    assert torch.equal(sample(logits, u, top_k=k.to(kt)), sample(logits, u, top_k=k.int()))
+    if kt in (torch.float32, torch.float16):
+        assert torch.equal(sample(logits, u, top_k=torch.full((5,), math.inf, device=dev, dtype=kt)), sample(logits, u))
