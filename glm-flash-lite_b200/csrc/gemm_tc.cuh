@@ -30,7 +30,8 @@ struct Epi
     int M, N;
     int bf16;                   // 16-bit type: bf16 or fp16
     int vec;                    // rows of every output can take 16-byte stores (always but for I8 with an odd width)
-    void* y; long long ldy; int y_dtype, accumulate;     // STORE, I8
+    void* y; long long ldy; int y_dtype;                 // STORE, I8
+    int accumulate;             // STORE
     void* o0; void* o1;         // GATED: o0 = h; DACT: o0 = dg, o1 = du; [M] rows of N, ldo apart
     long long ldo;
     float* p; float* q;         // [M][N]
@@ -51,14 +52,9 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, int bf16)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int W>
-__device__ __forceinline__ void store16(void* base, size_t off, const float (&v)[W], int bf16)
+__device__ __forceinline__ void store16(void* base, size_t off, const float (&v)[4], int bf16)
 {
-    uint32_t w[W / 2];
-#pragma unroll
-    for (int i = 0; i < W / 2; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], bf16);
-    uint8_t* d = static_cast<uint8_t*>(base) + off * 2;
-    *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(base) + off * 2) = make_uint2(pack16(v[0], v[1], bf16), pack16(v[2], v[3], bf16));
 }
 
 __device__ __forceinline__ float load16(const void* base, size_t off, int bf16)
@@ -66,12 +62,7 @@ __device__ __forceinline__ float load16(const void* base, size_t off, int bf16)
     return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[off]) : __half2float(static_cast<const __half*>(base)[off]);
 }
 
-template <int W>
-__device__ __forceinline__ void store_f32(float* d, const float (&v)[W])
-{
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i) reinterpret_cast<float4*>(d)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-}
+__device__ __forceinline__ void store_f32(float* d, const float (&v)[4]) { *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]); }
 
 // the two values of a 32-bit word, as a pair of fp32 registers
 template <bool BF16>
@@ -236,9 +227,9 @@ __device__ __forceinline__ void emit_gated(const Epi& e, int t, int n, const uin
         pp[i] = ku[i] ? ac : 0.0f;
         qq[i] = kg[i] ? up * (s[i] + act[i] * (1.0f - s[i])) : 0.0f;
     }
-    store16<4>(e.o0, (size_t) t * e.ldo + n, hh, e.bf16);
+    store16(e.o0, (size_t) t * e.ldo + n, hh, e.bf16);
     const size_t o = (size_t) t * e.N + n;
-    if (e.p) { store_f32<4>(e.p + o, pp); store_f32<4>(e.q + o, qq); }
+    if (e.p) { store_f32(e.p + o, pp); store_f32(e.q + o, qq); }
 }
 
 // W (4, or 1 where rows cannot take wide stores) consecutive columns n .. n + W - 1 of token t; n is a multiple of W. acc: the sums (I8: int32).
@@ -247,25 +238,21 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
 {
     if (t >= e.M || n >= e.N) return;
     float v[W];
-    if constexpr (EPI == EPI_DACT && W == 4)
+    if constexpr (EPI == EPI_DACT)
     {
         const size_t o = (size_t) t * e.N + n;
-        float dg[W], du[W];
+        const float4 p = *reinterpret_cast<const float4*>(e.p + o), q = *reinterpret_cast<const float4*>(e.q + o);
+        const float pv[4] = { p.x, p.y, p.z, p.w }, qv[4] = { q.x, q.y, q.z, q.w };
+        float dg[4], du[4];
 #pragma unroll
-        for (int i = 0; i < W / 4; ++i)
+        for (int i = 0; i < 4; ++i)
         {
-            const float4 p = *reinterpret_cast<const float4*>(e.p + o + 4 * i), q = *reinterpret_cast<const float4*>(e.q + o + 4 * i);
-            const float pv[4] = { p.x, p.y, p.z, p.w }, qv[4] = { q.x, q.y, q.z, q.w };
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-            {
-                const float d = __uint_as_float(acc[4 * i + j]);
-                dg[4 * i + j] = d * qv[j];
-                du[4 * i + j] = d * pv[j];
-            }
+            const float d = __uint_as_float(acc[i]);
+            dg[i] = d * qv[i];
+            du[i] = d * pv[i];
         }
-        store16<W>(e.o0, (size_t) t * e.ldo + n, dg, e.bf16);
-        store16<W>(e.o1, (size_t) t * e.ldo + n, du, e.bf16);
+        store16(e.o0, (size_t) t * e.ldo + n, dg, e.bf16);
+        store16(e.o1, (size_t) t * e.ldo + n, du, e.bf16);
         return;
     }
     if constexpr (EPI == EPI_I8)
@@ -286,14 +273,15 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
     }
     const size_t o = (size_t) t * e.ldy + n;
     const bool f32 = e.y_dtype == GLMX_F32, bf = e.y_dtype == GLMX_BF16;
+    const bool held = EPI == EPI_STORE && e.accumulate;
     if constexpr (W == 4)
         if (e.vec && n + W <= e.N)
         {
-            if (e.accumulate)
+            if (held)
 #pragma unroll
                 for (int i = 0; i < W; ++i) v[i] += f32 ? static_cast<const float*>(e.y)[o + i] : load16(e.y, o + i, bf);
-            if (f32) store_f32<W>(static_cast<float*>(e.y) + o, v);
-            else store16<W>(e.y, o, v, bf);
+            if (f32) store_f32(static_cast<float*>(e.y) + o, v);
+            else store16(e.y, o, v, bf);
             return;
         }
 #pragma unroll
@@ -303,11 +291,11 @@ __device__ __forceinline__ void emit(const Epi& e, int t, int n, const uint32_t 
         if (f32)
         {
             float* d = static_cast<float*>(e.y) + o + i;
-            *d = e.accumulate ? *d + v[i] : v[i];
+            *d = held ? *d + v[i] : v[i];
         }
         else
         {
-            const float w = e.accumulate ? load16(e.y, o + i, bf) + v[i] : v[i];
+            const float w = held ? load16(e.y, o + i, bf) + v[i] : v[i];
             if (bf) static_cast<__nv_bfloat16*>(e.y)[o + i] = __float2bfloat16_rn(w);
             else static_cast<__half*>(e.y)[o + i] = __float2half_rn(w);
         }
