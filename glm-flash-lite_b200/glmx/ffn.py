@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import check
@@ -54,7 +54,8 @@ def _rows(t: torch.Tensor, align: int, pitch_of_copy: int = 64) -> torch.Tensor:
 
 
 def _no_tangent(t: torch.Tensor) -> None:
-    if unpack_dual(t).tangent is not None:
+    # (outside of every level no tensor has one, which is cheaper to see)
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
         raise RuntimeError("the gated feed-forward block has no forward-mode derivative")
 
 
