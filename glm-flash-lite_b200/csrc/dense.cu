@@ -80,8 +80,7 @@ extern "C" int glmx_dense_check(void* stream, int* flags)
     if (e == cudaSuccess && v)
     {
         // the bits that are reported, no others: a kernel of another stream may have set one since
-        clear_kernel<<<1, 1, 0, st>>>(p, v);
-        e = cudaGetLastError();
+        e = dense_launch(clear_kernel, 1, 1, st, p, v);
         if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     }
     if (e != cudaSuccess) return dense_cuda_fail(e, "glmx_dense_check");

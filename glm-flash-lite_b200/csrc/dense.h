@@ -58,6 +58,18 @@ public:
     }
 };
 
+// A launch that returns its own error: cudaGetLastError after <<<>>> would also report one that an earlier call of the thread has
+// returned already.
+template <typename... P, typename... A>
+cudaError_t dense_launch(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t st, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // the dynamic shared memory that a kernel's launches may ask for, set once
 inline cudaError_t dense_smem(PerDevice<int>& set, int device, const void* kernel, int bytes)
 {

@@ -104,8 +104,8 @@ extern "C" int glmx_ffn_forward(const glmx_ffn* f, const void* x, long long ldx,
     if (p && g.e.limit != 0.0f && !accumulate && ldy == H && y_bytes >= 2 * rows && apart)
     {
         __nv_bfloat16* norms = static_cast<__nv_bfloat16*>(y);
-        norms_kernel<<<(unsigned) ((rows + NORM_WARPS - 1) / NORM_WARPS), NORM_WARPS * 32, 0, st>>>(f->w_gate, f->w_up, I, x, ldx, ntok, H, g.e.bf16, norms);
-        e = cudaGetLastError();
+        e = dense_launch(norms_kernel, (unsigned) ((rows + NORM_WARPS - 1) / NORM_WARPS), NORM_WARPS * 32, st, f->w_gate, f->w_up, I, x, ldx, ntok, H,
+                         g.e.bf16, norms);
         g.e.norms = norms;
     }
     if (e == cudaSuccess) e = launch_product<false, false, EPI_GATED>(f->dtype, g, 1, H, false, st);

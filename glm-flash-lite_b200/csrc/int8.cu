@@ -142,18 +142,18 @@ __global__ void __launch_bounds__(QT) quantize_any_kernel(const T* x, long long 
 }
 
 template <typename T>
-void launch_quantize(const void* xv, long long ldx, int rows, int K, signed char* q, long long ldq, float* scale, cudaStream_t st)
+cudaError_t launch_quantize(const void* xv, long long ldx, int rows, int K, signed char* q, long long ldq, float* scale, cudaStream_t st)
 {
     constexpr int G = 16 / sizeof(T);
     const T* x = static_cast<const T*>(xv);
     const int nv = (K / G + QT - 1) / QT;
-    if (K % G || ldx % G || !dense_aligned(x) || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || nv > 8)
-        quantize_any_kernel<T><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
-    else if (nv == 1) quantize_kernel<T, 1><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
-    else if (nv == 2) quantize_kernel<T, 2><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
-    else if (nv == 3) quantize_kernel<T, 3><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
-    else if (nv == 4) quantize_kernel<T, 4><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
-    else quantize_kernel<T, 8><<<rows, QT, 0, st>>>(x, ldx, K, q, ldq, scale);
+    auto kernel = quantize_kernel<T, 8>;
+    if (K % G || ldx % G || !dense_aligned(x) || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8 || nv > 8) kernel = quantize_any_kernel<T>;
+    else if (nv == 1) kernel = quantize_kernel<T, 1>;
+    else if (nv == 2) kernel = quantize_kernel<T, 2>;
+    else if (nv == 3) kernel = quantize_kernel<T, 3>;
+    else if (nv == 4) kernel = quantize_kernel<T, 4>;
+    return dense_launch(kernel, (unsigned) rows, QT, st, x, ldx, K, q, ldq, scale);
 }
 
 }  // namespace
@@ -171,10 +171,9 @@ extern "C" int glmx_quantize_rows(const void* x, int x_dtype, long long ldx, int
     if (rows == 0) return GLMX_OK;
     if (!x || !q || !scale) return dense_fail(GLMX_E_ARG, "glmx_quantize_rows: null argument");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (x_dtype == GLMX_F32) launch_quantize<float>(x, ldx, rows, K, q, ldq, scale, st);
-    else if (x_dtype == GLMX_F16) launch_quantize<__half>(x, ldx, rows, K, q, ldq, scale, st);
-    else launch_quantize<__nv_bfloat16>(x, ldx, rows, K, q, ldq, scale, st);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = x_dtype == GLMX_F32 ? launch_quantize<float>(x, ldx, rows, K, q, ldq, scale, st)
+                        : x_dtype == GLMX_F16 ? launch_quantize<__half>(x, ldx, rows, K, q, ldq, scale, st)
+                                              : launch_quantize<__nv_bfloat16>(x, ldx, rows, K, q, ldq, scale, st);
     return e == cudaSuccess ? GLMX_OK : dense_cuda_fail(e, "glmx_quantize_rows: launch");
 }
 

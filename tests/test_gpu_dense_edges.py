@@ -454,3 +454,22 @@ def test_sample_top_k_of_any_type(dev, kt):
     assert torch.equal(sample(logits, u, top_k=k.to(kt)), sample(logits, u, top_k=k.int()))
     if kt in (torch.float32, torch.float16):
         assert torch.equal(sample(logits, u, top_k=torch.full((5,), math.inf, device=dev, dtype=kt)), sample(logits, u))
+
+
+def test_errors_of_earlier_calls_are_not_reported_again(dev):
+    """A call that failed (here an allocation beyond the device's memory) has returned its error; the next ones succeed."""
+    import ctypes as C
+    from glmx import GatedFFN, Int8Linear, _lib, dense_check, quantize_rows, sample
+    L = _lib.load()
+    x, wg, wu, wd, dy = block(dev, 5, 128, 64, BF, 931)
+    ffn, lin = GatedFFN(wg, wu, wd, act_limit=1.0), Int8Linear.from_weight(wg)
+    u = torch.rand(5, device=dev)
+
+    def train():
+        return ffn.backward(dy, ffn.forward_train(x)[1])[0]
+    for call in (lambda: quantize_rows(x)[0], lambda: quantize_rows(x[:, 1:])[0], lambda: ffn(x), train, lambda: lin(x), lambda: sample(x, u)):
+        want = call()
+        assert L.glmx_ipc_alloc(1 << 60, C.byref(C.c_void_p())) == _lib.E_CUDA
+        assert torch.equal(call(), want)
+    assert L.glmx_ipc_alloc(1 << 60, C.byref(C.c_void_p())) == _lib.E_CUDA
+    dense_check()
