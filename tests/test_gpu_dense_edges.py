@@ -473,3 +473,24 @@ def test_errors_of_earlier_calls_are_not_reported_again(dev):
         assert torch.equal(call(), want)
     assert L.glmx_ipc_alloc(1 << 60, C.byref(C.c_void_p())) == _lib.E_CUDA
     dense_check()
+
+
+@pytest.mark.parametrize("T", [2, 17, 100, 300, 1100])
+def test_rows_do_not_depend_on_their_place(dev, T):
+    """A batch's rows in another order give the same rows' bits, in that order."""
+    from glmx import GatedFFN, Int8Linear, quantize_rows, sample
+    x, wg, wu, wd, dy = block(dev, T, 1024, 520, BF, 941 + T)
+    gen = torch.Generator(device=dev).manual_seed(T)
+    perm = torch.randperm(T, generator=gen, device=dev)
+    u = torch.rand(T, generator=gen, device=dev)
+    for L in (0.0, 1.25):
+        ffn = GatedFFN(wg, wu, wd, act_limit=L)
+        y, saved = ffn.forward_train(x)
+        yp, saved_p = ffn.forward_train(x[perm])
+        assert torch.equal(yp, y[perm]) and torch.equal(ffn(x[perm]), y[perm])
+        assert torch.equal(ffn.backward(dy[perm], saved_p)[0], ffn.backward(dy, saved)[0][perm])
+    lin = Int8Linear.from_weight(wg, out_dtype=F32)
+    logits = lin(x)
+    assert torch.equal(lin(x[perm]), logits[perm])
+    assert all(torch.equal(a, b[perm]) for a, b in zip(quantize_rows(x[perm]), quantize_rows(x)))
+    assert torch.equal(sample(logits[perm], u[perm], top_p=0.9), sample(logits, u, top_p=0.9)[perm])
