@@ -68,8 +68,9 @@ struct Weight
         // never 0, also where T is infinite: -inf * 0 would be NaN
         c = (float) fmax(fmin(2.8853900817779268 / (double) T, 3e38), 0x1p-149);
     }
-    // floor(2^44 2^((l - m) / T log2(e))), of half the difference, which no two finite logits overflow. The exponent's rounding moves a weight of
-    // 2^-x by x 2^-24 of itself, the exponential by about 2^-22: no more than fp32 logits carry. -inf gives 0 at every temperature
+    // floor(2^44 2^((l - m) / T log2(e))), of half the difference, which no two finite logits overflow. The exponent's three roundings
+    // (the difference, the scale, their product) move a weight of 2^-x by x 2^-23 of itself, the exponential by 2^-22: no more than the last bits of
+    // fp32 logits of that distance do. -inf gives 0 at every temperature
     __device__ __forceinline__ u64 operator()(float l) const
     {
         float e;
@@ -225,7 +226,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const __grid_constant__ S
     {
         // the row of this cluster: those with a top-p but no small top-k first, then those without either, then the others: a row of the
         // first kind that starts when others have ended is what the call waits for (64 rows of 150001, 13 of them of that kind: 54 us, 66 in
-        // the rows' order)
+        // the rows' order). A thread sorts a row: with more rows than threads they are taken in order, and what a row of the first kind
+        // takes is then a smaller part of the call
         int c = 3;
         if (tid < (int) gridDim.y)
         {

@@ -31,7 +31,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     descending order, each whose predecessors hold less than top_p of the weight left (1: all); of those, each with at
     least min_p times the largest weight; the largest always. The pick is the lowest id at which the running sum of the
     kept weights, in id order, exceeds u times their sum. temperature 0 picks the largest logit (the lowest id of equal
-    ones). -inf and NaN logits are never picked; a row without any other gives -1.
+    ones). -inf and NaN logits are never picked; a row without any other gives -1. An infinite temperature gives
+    all others the same weight.
 
     temperature, top_k, top_p and min_p: one number for all rows, or a tensor [B]."""
     if logits.dim() != 2 or logits.shape[1] < 1:

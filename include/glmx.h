@@ -312,7 +312,7 @@ GLMX_API int glmx_ffn_forward(const glmx_ffn* ffn, const void* x, long long ldx,
 /* Gradients of glmx_ffn_forward (accumulate = 0) for dy [ntok][H] (rows lddy apart), from the x, h, p and q of the forward call: dx
  * [ntok][H], dw_gate / dw_up [I][H], dw_down [H][I], all in the block's dtype, rows packed; a NULL one is not computed.
  * dg, du: caller's scratch like h, one each (the gradients of g and u afterwards); not needed (NULL) where only
- * dw_down is asked for. */
+ * dw_down is asked for. No output may overlap an input. */
 GLMX_API int glmx_ffn_backward(const glmx_ffn* ffn, const void* dy, long long lddy, const void* x, long long ldx, int ntok,
                                const void* h, const float* p, const float* q, void* dg, void* du, void* dx, void* dw_gate,
                                void* dw_up, void* dw_down, void* stream);
@@ -340,8 +340,9 @@ GLMX_API int glmx_linear_i8(const signed char* xq, long long ldxq, const float* 
  *   the kept weights, in id order, exceeds u * their sum.
  * temperature <= 0 picks the largest logit (ties to the lower id). A logit of -inf or NaN is never picked; a row that has no other gives -1.
  * Equal +inf logits share the weight. temperature, top_k, top_p, min_p: device arrays [B], or NULL for the value behind
- * (one for all rows). ids: [B] GLMX_I32 or GLMX_I64. Weights are exponentials in fp32 (a few ulp) rounded to multiples of
- * 2^-44 and summed as 64-bit integers, so a call's result does not depend on the order of summation. */
+ * (one for all rows). ids: [B] GLMX_I32 or GLMX_I64. Weights are exponentials in fp32 (one of 2^-x is within (x + 2) 2^-23
+ * of itself) rounded down to multiples of 2^-44 and summed as 64-bit integers, so a call's result does not depend on the order of summation.
+ * An infinite temperature gives all logits but -inf and NaN the same weight. */
 #define GLMX_SAMPLE_MAX_VOCAB 393216
 GLMX_API int glmx_sample(const void* logits, int dtype, long long ld, int B, int V, const float* u, const float* temperature,
                          float temperature0, const int* top_k, int top_k0, const float* top_p, float top_p0,
